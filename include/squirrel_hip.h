@@ -263,6 +263,83 @@ int sq_softmax(const float* d_in, float* d_out, size_t n);
  * idx >= n is SQ_ERR_ARG (the reference would panic on the index). */
 int sq_log_softmax_at(const float* d_logits, size_t n, uint32_t idx, double* out);
 
+/* ---- a serving step over a paged key/value cache in 8 bits -------------
+ * No counterpart in the reference, whose cache is one sequence's f32 rows
+ * (kv_cache.rs:1-16).  A pool holds pages of SQ_KV_PAGE positions for every
+ * layer; a page belongs to one sequence at a time and the caller's page tables
+ * say which (page t of a sequence's table holds its positions 64 t .. 64 t + 63).
+ * Keys and values are stored as 8-bit integers q with one f32 scale s for each
+ * (page, KV head), keys and values apart: the cached value is q * s.
+ *
+ * One step: describe it once in a plan, then for every layer append the new
+ * keys and values and attend.  Calls run on the null stream and return
+ * finished.  A plan belongs to one thread at a time; a pool may be shared by
+ * plans whose steps write different pages.  Free plans before their pool.  Every call needs the
+ * pool's device to be the current one (SQ_ERR_ARG otherwise). */
+#define SQ_KV_PAGE 64
+#define SQ_KV_ROTATED 1u /* the rows are rotated already */
+typedef struct sq_kv_pool sq_kv_pool;
+typedef struct sq_kv_plan sq_kv_plan;
+/* head_dim is 64 or 128 (SQ_ERR_UNSUPPORTED otherwise).  inv_freq (half
+ * floats of host memory, half <= head_dim / 2): the rotation of queries and
+ * keys, pairs (2j, 2j + 1) by position * inv_freq[j] as in sq_rope_rows, the
+ * angle in 64 bits (sq_rope_rows rounds it to f32 as the reference does, off
+ * by up to 2^-24 of the angle); dimensions past 2 * half stay as they are.
+ * Pages start as zeros. */
+int sq_kv_pool_new(size_t n_layers, size_t n_pages, size_t n_kv_heads, size_t head_dim,
+                   const float* inv_freq, size_t half, sq_kv_pool** out);
+void sq_kv_pool_free(sq_kv_pool* pool);
+int sq_kv_plan_new(const sq_kv_pool* pool, sq_kv_plan** out);
+/* The step's sequences (all host memory): past[i] positions cached before it,
+ * n_new[i] >= 0 rows of it, and a row of `tables` (table_stride entries) with
+ * at least the pages of past[i] + n_new[i] positions.  The batch's rows are
+ * sequence 0's, then sequence 1's, and so on.  A page past the pool, or one
+ * that the step writes and that stands in the tables a second time, is
+ * SQ_ERR_ARG (pages that are only read may be shared).  past[i] may be less
+ * than an earlier step left: drafts that were rejected are overwritten.  A
+ * refused call leaves the plan's former step in place. */
+int sq_kv_plan_set(sq_kv_plan* plan, size_t n_seqs, const uint32_t* past, const uint32_t* n_new,
+                   const uint32_t* tables, size_t table_stride);
+void sq_kv_plan_free(sq_kv_plan* plan);
+/* Rotates the batch's keys (not with SQ_KV_ROTATED), quantizes keys and
+ * values and writes them.  Strides in floats, at least kv_heads * head_dim.
+ * The scale of a page whose first row is new is f32(max|x| / 127) over its new rows;
+ * behind earlier rows it is that or the page's former scale, whichever is larger, and
+ * where it grows the earlier rows' integers become rint(q * s_old / s).  A
+ * value x is stored as rint(x / s).  A row that is not finite is SQ_ERR_ARG: it is
+ * stored as zero (a key's whole pair), everything else of the call as it should be. */
+int sq_kv_append(sq_kv_plan* plan, size_t layer, const float* d_k, size_t k_stride,
+                 const float* d_v, size_t v_stride, uint32_t flags);
+/* The cached values of the last min(last, past + n_new) positions of every
+ * sequence, sequence after sequence, rows of kv_heads * head_dim floats; either
+ * output may be null. */
+int sq_kv_read(sq_kv_plan* plan, size_t layer, size_t last, float* d_k, float* d_v);
+/* Attention of the batch's rows, appended before, over their sequences: d_q
+ * (rotated on the way, not with SQ_KV_ROTATED) and d_out hold n_heads *
+ * head_dim floats a row, strides in floats.  A query at position p sees the
+ * positions j <= p, with a window (> 0) those with j > p - window or j <
+ * n_sinks.  f32 results as sq_sdpa's over the cached values.  d_out may be d_q. */
+int sq_sdpa_paged(sq_kv_plan* plan, size_t layer, const float* d_q, size_t q_stride, float* d_out,
+                  size_t out_stride, size_t n_heads, size_t window, size_t n_sinks,
+                  uint32_t flags);
+/* Verification of drafted tokens.  Sequence i has n_draft[i] drafts (host
+ * memory, at most 1024, 0 allowed): n_draft[i] rows of draft logits, ids
+ * d_tokens and n_draft[i] + 1 rows of target logits and numbers d_u in [0, 1),
+ * each sequence after sequence; strides in floats.  With p = softmax(target /
+ * temperature) and q = softmax(draft / temperature) (d_draft null: the draft's
+ * token has probability 1), draft x_j is accepted while u_j q_j(x_j) < p_j(x_j);
+ * accepted[i] counts them and next[i] is drawn with the sequence's last number u:
+ * the smallest t at which the running sum of the weights max(p_j - q_j, 0) of the
+ * first rejected draft, or of p behind the last, exceeds u times their total.
+ * Temperature 0: accepted while a draft is sq_greedy's token, next is sq_greedy's.
+ * In 64 bits throughout.  Logits may be -inf (probability 0); a row on which the
+ * result depends that holds NaN or +inf or nothing above -inf, or an id past the
+ * vocabulary, is SQ_ERR_ARG, and the results are left as they were. */
+int sq_verify_draft(const float* d_target, size_t target_stride, const float* d_draft,
+                    size_t draft_stride, const uint32_t* d_tokens, const float* d_u,
+                    const uint32_t* n_draft, size_t n_seqs, size_t vocab, float temperature,
+                    uint32_t* accepted, uint32_t* next);
+
 /* ---- measurement -----------------------------------------------------
  * Replays one kernel of the context's decode step `iters` times on the
  * context stream between two HIP events and returns the mean duration.

@@ -1,11 +1,15 @@
 // extern "C" entry points declared in include/squirrel_hip.h.
+#include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <new>
 #include <string>
 #include <vector>
 
+#include "kv.h"
 #include "model.h"
 #include "scratch.h"
+#include "verify.h"
 
 namespace sq {
 
@@ -518,6 +522,169 @@ int sq_greedy(const float* d_logits, size_t n, uint32_t* token) {
         return st;
     if ((st = finish(0))) return st;
     SQ_HIP_CHECK(hipMemcpy(token, tok.p, 4, hipMemcpyDeviceToHost));
+    return 0;
+}
+
+// ------------------------------------------------------------ paged 8-bit cache
+
+int sq_kv_pool_new(size_t n_layers, size_t n_pages, size_t n_kv_heads, size_t head_dim, const float* inv_freq,
+                   size_t half, sq_kv_pool** out) {
+    if (!out) return set_error(SQ_ERR_ARG, "kv_pool: null argument");
+    return kv_pool_create(n_layers, n_pages, n_kv_heads, head_dim, inv_freq, half, out);
+}
+
+void sq_kv_pool_free(sq_kv_pool* pool) { kv_pool_destroy(pool); }
+
+int sq_kv_plan_new(const sq_kv_pool* pool, sq_kv_plan** out) {
+    if (!pool || !out) return set_error(SQ_ERR_ARG, "kv_plan: null argument");
+    return kv_plan_create(pool, out);
+}
+
+int sq_kv_plan_set(sq_kv_plan* plan, size_t n_seqs, const uint32_t* past, const uint32_t* n_new,
+                   const uint32_t* tables, size_t table_stride) {
+    if (!plan) return set_error(SQ_ERR_ARG, "kv_plan: null argument");
+    return kv_plan_fill(plan, n_seqs, past, n_new, tables, table_stride);
+}
+
+void sq_kv_plan_free(sq_kv_plan* plan) { kv_plan_destroy(plan); }
+
+int sq_kv_append(sq_kv_plan* plan, size_t layer, const float* d_k, size_t k_stride, const float* d_v, size_t v_stride,
+                 uint32_t flags) {
+    if (!plan) return set_error(SQ_ERR_ARG, "kv_append: null plan");
+    if (flags & ~SQ_KV_ROTATED) return set_error(SQ_ERR_ARG, "kv_append: unknown flag");
+    const size_t width = plan->pool->kv_heads * plan->pool->head_dim;
+    if (k_stride < width || v_stride < width)
+        return set_error(SQ_ERR_SHAPE, "kv_append: ShapeMismatch (rows shorter than the pool's)");
+    KvView kv;
+    KvPlanView pv;
+    int st = kv_views(plan, layer, !(flags & SQ_KV_ROTATED), "kv_append", &kv, &pv);
+    if (st) return finish(st);
+    if (pv.rows == 0) return 0;
+    if (!d_k || !d_v) return finish(set_error(SQ_ERR_ARG, "kv_append: null argument"));
+    *plan->bad = 0;
+    if ((st = finish(launch_kv_append(nullptr, kv, pv, d_k, k_stride, d_v, v_stride, plan->bad)))) return st;
+    if (*(volatile uint32_t*)plan->bad)
+        return set_error(SQ_ERR_ARG, "kv_append: a key or value is not finite (stored as zero)");
+    return 0;
+}
+
+int sq_kv_read(sq_kv_plan* plan, size_t layer, size_t last, float* d_k, float* d_v) {
+    if (!plan) return set_error(SQ_ERR_ARG, "kv_read: null plan");
+    KvView kv;
+    KvPlanView pv;
+    if (int st = kv_views(plan, layer, false, "kv_read", &kv, &pv)) return st;
+    const int most = (int)std::min<size_t>(last, INT32_MAX);
+    int pages = 0;
+    for (const KvSeq& s : plan->seqs) {
+        const int len = s.past + s.n_new, first = len > most ? len - most : 0;
+        if (first < len) pages = std::max(pages, (len - 1) / kPage - first / kPage + 1);
+    }
+    if (pages == 0) return 0;
+    if (!d_k && !d_v) return set_error(SQ_ERR_ARG, "kv_read: null argument");
+    return finish(launch_kv_read(nullptr, kv, pv, most, pages, d_k, d_v));
+}
+
+int sq_sdpa_paged(sq_kv_plan* plan, size_t layer, const float* d_q, size_t q_stride, float* d_out, size_t out_stride,
+                  size_t n_heads, size_t window, size_t n_sinks, uint32_t flags) {
+    if (!plan) return set_error(SQ_ERR_ARG, "sdpa_paged: null plan");
+    if (flags & ~SQ_KV_ROTATED) return set_error(SQ_ERR_ARG, "sdpa_paged: unknown flag");
+    if (n_heads == 0 || n_heads > 65535 || n_heads % plan->pool->kv_heads)
+        return set_error(SQ_ERR_SHAPE, "sdpa_paged: ShapeMismatch (heads)");
+    const size_t width = n_heads * plan->pool->head_dim;
+    if (q_stride < width || out_stride < width)
+        return set_error(SQ_ERR_SHAPE, "sdpa_paged: ShapeMismatch (rows shorter than the heads)");
+    KvView kv;
+    KvPlanView pv;
+    int st = kv_views(plan, layer, !(flags & SQ_KV_ROTATED), "sdpa_paged", &kv, &pv);
+    if (st) return finish(st);
+    if (pv.rows == 0) return 0;
+    if (!d_q || !d_out) return finish(set_error(SQ_ERR_ARG, "sdpa_paged: null argument"));
+    size_t longest = 0;
+    for (const KvSeq& s : plan->seqs) longest = std::max(longest, (size_t)s.past + s.n_new);
+    // (a window that reaches over every sequence is none)
+    const PagedArgs a{d_q,        q_stride,     d_out,
+                      out_stride, (int)n_heads, window < longest ? (int)window : 0,
+                      (int)std::min(n_sinks, longest)};
+    Tmp ws;
+    const size_t floats = sdpa_paged_floats(plan->seqs, kv, a);
+    if (floats && (st = ws.alloc(floats * sizeof(float)))) return finish(st);
+    return finish(launch_sdpa_paged(nullptr, plan->seqs, kv, pv, a, (float*)ws.p));
+}
+
+int sq_verify_draft(const float* d_target, size_t target_stride, const float* d_draft, size_t draft_stride,
+                    const uint32_t* d_tokens, const float* d_u, const uint32_t* n_draft, size_t n_seqs, size_t vocab,
+                    float temperature, uint32_t* accepted, uint32_t* next) {
+    if (n_seqs == 0) return 0;
+    if (!n_draft || !accepted || !next || !d_target || !d_u)
+        return set_error(SQ_ERR_ARG, "verify_draft: null argument");
+    if (vocab == 0) return set_error(SQ_ERR_EMPTY, "verify_draft: EmptyInput");
+    if (vocab > (size_t)INT32_MAX / 2) return set_error(SQ_ERR_SHAPE, "verify_draft: ShapeMismatch (row too long)");
+    if (!(temperature >= 0.0f && temperature < INFINITY))
+        return set_error(SQ_ERR_ARG, "verify_draft: the temperature is not a finite number of at least 0");
+    if (n_seqs > ((size_t)1 << 24)) return set_error(SQ_ERR_SHAPE, "verify_draft: ShapeMismatch (too many sequences)");
+    size_t drafts = 0;
+    for (size_t i = 0; i < n_seqs; i++) {
+        if (n_draft[i] > kVerifyDrafts) return set_error(SQ_ERR_SHAPE, "verify_draft: ShapeMismatch (more than 1024 drafts)");
+        drafts += n_draft[i];
+    }
+    if (target_stride < vocab || (d_draft && draft_stride < vocab))
+        return set_error(SQ_ERR_SHAPE, "verify_draft: ShapeMismatch (rows shorter than the vocabulary)");
+    if (drafts && !d_tokens) return set_error(SQ_ERR_ARG, "verify_draft: null argument");
+    const bool with_draft = d_draft && temperature > 0.0f;
+    Tmp res, ws;
+    int st;
+    if ((st = res.alloc(n_seqs * sizeof(VerifyResult)))) return st;
+    std::vector<VerifyResult> host;
+    try {
+        host.resize(n_seqs);
+    } catch (const std::bad_alloc&) {
+        return set_error(SQ_ERR_ARG, "verify_draft: out of host memory");
+    }
+    // batches of sequences whose counts fit a launch's arguments; the
+    // workspace of one serves the next (the null stream orders them)
+    size_t t0 = 0, d0 = 0;
+    for (size_t s0 = 0; s0 < n_seqs;) {
+        VerifyBatch b;
+        memset(&b, 0, sizeof(b));
+        size_t rows = 0;
+        while (b.n_seqs < (uint32_t)kVerifySeqs && s0 + b.n_seqs < n_seqs) {
+            b.target0[b.n_seqs] = (uint32_t)rows;
+            b.n[b.n_seqs] = (uint16_t)n_draft[s0 + b.n_seqs];
+            rows += n_draft[s0 + b.n_seqs] + 1;
+            b.n_seqs++;
+        }
+        const size_t n_rows = rows - b.n_seqs;
+        const VerifyArgs a{d_target + t0 * target_stride,
+                           target_stride,
+                           with_draft ? d_draft + d0 * draft_stride : nullptr,
+                           draft_stride,
+                           drafts ? d_tokens + d0 : d_tokens,
+                           d_u + t0,
+                           (int)vocab,
+                           temperature > 0.0f ? 1.4426950408889634074 / (double)temperature : 0.0};
+        const size_t bytes = verify_ws_bytes(rows + (with_draft ? n_rows : 0), b.n_seqs, (int)vocab);
+        if (ws.p && ws.size < bytes) {
+            scratch_put(ws.p, ws.size, ws.device);
+            ws.p = nullptr;
+        }
+        if (!ws.p && (st = ws.alloc(bytes))) return finish(st);
+        if ((st = launch_verify(nullptr, b, a, rows, with_draft ? n_rows : 0, ws.p, (VerifyResult*)res.p + s0)))
+            return finish(st);
+        s0 += b.n_seqs;
+        t0 += rows;
+        d0 += n_rows;
+    }
+    if ((st = finish(0))) return st;
+    SQ_HIP_CHECK(hipMemcpy(host.data(), res.p, n_seqs * sizeof(VerifyResult), hipMemcpyDeviceToHost));
+    for (size_t i = 0; i < n_seqs; i++) {
+        if (host[i].bad == 1)
+            return set_error(SQ_ERR_ARG, "verify_draft: logits of sequence " + std::to_string(i) +
+                                             " hold NaN or +inf, or nothing above -inf");
+        if (host[i].bad)
+            return set_error(SQ_ERR_ARG, "verify_draft: a drafted token of sequence " + std::to_string(i) +
+                                             " is past the vocabulary");
+    }
+    for (size_t i = 0; i < n_seqs; i++) accepted[i] = host[i].accepted, next[i] = host[i].token;
     return 0;
 }
 

@@ -17,6 +17,7 @@ SQ_ERR_UNSUPPORTED, SQ_ERR_CACHE_FULL, SQ_ERR_ARG, SQ_ERR_HIP = 20, 21, 22, 64
 SQ_F32, SQ_Q4_0, SQ_Q8_0, SQ_BF16 = 0, 2, 8, 30
 SQ_CTX_F32_ACTS, SQ_CTX_NO_GRAPH, SQ_CTX_MULTI_KERNEL = 1, 2, 4
 SQ_GEN_IGNORE_EOS, SQ_GEN_NO_KV_CACHE = 1, 2
+SQ_KV_PAGE, SQ_KV_ROTATED = 64, 1
 
 
 class SynthSpec(C.Structure):
@@ -90,6 +91,15 @@ PROTOS = {
     "sq_gemm_tile64x128_launches": ([vp], i32),
     "sq_device_wall_clock_khz": ([vp], i32),
     "sq_log_softmax_at": ([vp, sz, u32, vp], i32),
+    "sq_kv_pool_new": ([sz, sz, sz, sz, vp, sz, C.POINTER(vp)], i32),
+    "sq_kv_pool_free": ([vp], None),
+    "sq_kv_plan_new": ([vp, C.POINTER(vp)], i32),
+    "sq_kv_plan_set": ([vp, sz, vp, vp, vp, sz], i32),
+    "sq_kv_plan_free": ([vp], None),
+    "sq_kv_append": ([vp, sz, vp, sz, vp, sz, u32], i32),
+    "sq_kv_read": ([vp, sz, sz, vp, vp], i32),
+    "sq_sdpa_paged": ([vp, sz, vp, sz, vp, sz, sz, sz, sz, u32], i32),
+    "sq_verify_draft": ([vp, sz, vp, sz, vp, vp, vp, sz, sz, f32, vp, vp], i32),
     "sq_ctx_prefill_phases": ([vp, vp, sz, vp], i32),
 }
 

@@ -9,7 +9,7 @@ import ctypes as C
 
 import numpy as np
 
-from ._lib import SQ_CTX_F32_ACTS, check, lib
+from ._lib import SQ_CTX_F32_ACTS, SQ_KV_PAGE, SQ_KV_ROTATED, check, lib
 
 BLOCK_Q8_0 = np.dtype([("d", "<u2"), ("qs", "i1", (32,))])
 BLOCK_Q4_0 = np.dtype([("d", "<u2"), ("qs", "u1", (16,))])
@@ -206,3 +206,114 @@ def greedy(logits: DeviceArray) -> int:
     t = C.c_uint32()
     check(lib().sq_greedy(logits.ptr, logits.size, C.byref(t)))
     return t.value
+
+
+# ------------------------------------------------------ paged 8-bit cache
+
+
+class KvPool:
+    """Pages of SQ_KV_PAGE positions for `n_layers` layers, keys and values in
+    8 bits with a scale per page and KV head (sq_kv_pool_new).  inv_freq: the
+    rotation of keys and queries, None for none."""
+
+    def __init__(self, n_layers: int, n_pages: int, n_kv_heads: int, head_dim: int, inv_freq=None):
+        inv = np.ascontiguousarray(inv_freq if inv_freq is not None else [], dtype=np.float32)
+        self.n_kv_heads, self.head_dim = n_kv_heads, head_dim
+        self.h = None
+        h = C.c_void_p()
+        check(lib().sq_kv_pool_new(n_layers, n_pages, n_kv_heads, head_dim, inv.ctypes.data, inv.size, C.byref(h)))
+        self.h = h.value
+
+    def __del__(self):
+        try:
+            if self.h:
+                lib().sq_kv_pool_free(self.h)
+                self.h = None
+        except Exception:
+            pass
+
+
+class KvPlan:
+    """The sequences of one step over a pool (sq_kv_plan_set): positions cached
+    before it, rows of it, and the page table of each."""
+
+    def __init__(self, pool: KvPool, past=None, new=None, tables=None):
+        self.pool, self.rows, self.lengths, self.h = pool, 0, np.zeros(0, np.int64), None
+        h = C.c_void_p()
+        check(lib().sq_kv_plan_new(pool.h, C.byref(h)))
+        self.h = h.value
+        if past is not None:
+            self.set(past, new, tables)
+
+    def set(self, past, new, tables) -> None:
+        past, new, tables = np.asarray(past), np.asarray(new), np.asarray(tables)
+        if past.ndim != 1 or new.shape != past.shape or tables.ndim != 2 or len(tables) != len(past):
+            _shape_error()
+        for a in (past, new, tables):
+            if a.size and (a.min() < 0 or a.max() > 0xFFFFFFFF):
+                _shape_error()
+        p, n, t = (np.ascontiguousarray(a, dtype=np.uint32) for a in (past, new, tables))
+        check(lib().sq_kv_plan_set(self.h, len(p), p.ctypes.data, n.ctypes.data, t.ctypes.data, t.shape[1]))
+        self.rows, self.lengths = int(n.astype(np.int64).sum()), p.astype(np.int64) + n
+
+    def __del__(self):
+        try:
+            if self.h:
+                lib().sq_kv_plan_free(self.h)
+                self.h = None
+        except Exception:
+            pass
+
+
+def _row_stride(plan_rows: int, width: int, t, stride) -> int:
+    """Floats from row to row of t: `stride`, or those of a packed array."""
+    if stride is None:
+        if t.size != plan_rows * width:
+            _shape_error()
+        return width
+    return stride
+
+
+def kv_append(plan: KvPlan, layer: int, k: DeviceArray, v: DeviceArray, rotated: bool = False, k_stride=None,
+              v_stride=None) -> None:
+    """Rotates, quantizes and stores the step's keys and values (sq_kv_append).
+    k and v hold the step's rows, packed or `stride` floats apart."""
+    width = plan.pool.n_kv_heads * plan.pool.head_dim
+    check(lib().sq_kv_append(plan.h, layer, k.ptr, _row_stride(plan.rows, width, k, k_stride), v.ptr,
+                             _row_stride(plan.rows, width, v, v_stride), SQ_KV_ROTATED if rotated else 0))
+
+
+def kv_read(plan: KvPlan, layer: int, last: int, k: DeviceArray, v: DeviceArray) -> None:
+    """The cached values of each sequence's last `last` positions (sq_kv_read)."""
+    n = int(np.minimum(plan.lengths, last).sum()) * plan.pool.n_kv_heads * plan.pool.head_dim
+    if k.size != n or v.size != n:
+        _shape_error()
+    check(lib().sq_kv_read(plan.h, layer, last, k.ptr, v.ptr))
+
+
+def sdpa_paged(plan: KvPlan, layer: int, q: DeviceArray, out: DeviceArray, n_heads: int, window: int = 0,
+               sinks: int = 0, rotated: bool = False, q_stride=None, out_stride=None) -> None:
+    """Attention of the step's rows over the cache (sq_sdpa_paged)."""
+    width = n_heads * plan.pool.head_dim
+    check(lib().sq_sdpa_paged(plan.h, layer, q.ptr, _row_stride(plan.rows, width, q, q_stride), out.ptr,
+                              _row_stride(plan.rows, width, out, out_stride), n_heads, window, sinks,
+                              SQ_KV_ROTATED if rotated else 0))
+
+
+def verify_draft(target: DeviceArray, draft: DeviceArray | None, tokens: DeviceArray, u: DeviceArray, n_draft,
+                 temperature: float) -> tuple[np.ndarray, np.ndarray]:
+    """Accepted drafts and the next token of each sequence (sq_verify_draft)."""
+    n = np.asarray(n_draft)
+    if n.ndim != 1 or (n.size and (n.min() < 0 or n.max() > 0xFFFFFFFF)):
+        _shape_error()
+    n = np.ascontiguousarray(n, dtype=np.uint32)
+    drafts = int(n.astype(np.int64).sum())
+    if len(target.shape) != 2 or target.shape[0] != drafts + n.size or tokens.size != drafts or u.size != drafts + n.size:
+        _shape_error()
+    vocab = target.shape[1]
+    if draft is not None and draft.shape != (drafts, vocab):
+        _shape_error()
+    accepted, token = np.zeros(n.size, np.uint32), np.zeros(n.size, np.uint32)
+    check(lib().sq_verify_draft(target.ptr, vocab, draft.ptr if draft is not None else None, vocab, tokens.ptr, u.ptr,
+                                n.ctypes.data, n.size, vocab, temperature, accepted.ctypes.data, token.ctypes.data))
+    return accepted, token

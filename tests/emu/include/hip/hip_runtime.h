@@ -48,11 +48,14 @@ struct alignas(16) float4 { float x, y, z, w; };
 struct alignas(8) int2 { int x, y; };
 struct alignas(16) int4 { int x, y, z, w; };
 struct alignas(8) uint2 { unsigned x, y; };
+struct alignas(16) uint4 { unsigned x, y, z, w; };
+struct alignas(16) double2 { double x, y; };
 inline float2 make_float2(float a, float b) { return float2{a, b}; }
 inline float4 make_float4(float a, float b, float c, float d) { return float4{a, b, c, d}; }
 inline int2 make_int2(int a, int b) { return int2{a, b}; }
 inline int4 make_int4(int a, int b, int c, int d) { return int4{a, b, c, d}; }
 inline uint2 make_uint2(unsigned a, unsigned b) { return uint2{a, b}; }
+inline uint4 make_uint4(unsigned a, unsigned b, unsigned c, unsigned d) { return uint4{a, b, c, d}; }
 
 struct dim3 {
     unsigned x, y, z;
@@ -387,6 +390,12 @@ template <typename T>
 inline T atomicMax(T* p, T v) {
     T o = *p;
     if (v > o) *p = v;
+    return o;
+}
+template <typename T>
+inline T atomicMin(T* p, T v) {
+    T o = *p;
+    if (v < o) *p = v;
     return o;
 }
 
