@@ -193,6 +193,17 @@ inline int sdot4(int a, int b, int c, bool clamp) {
     return s;
 }
 
+// v_perm_b32: byte i of the result is byte sel_i of {s1 (0-3), s0 (4-7)}.
+inline unsigned perm(unsigned s0, unsigned s1, unsigned sel) {
+    unsigned r = 0;
+    for (int i = 0; i < 4; i++) {
+        const unsigned k = (sel >> (8 * i)) & 0xff;
+        if (k > 7) fatal("v_perm_b32: selector %u is not emulated", k);
+        r |= ((k < 4 ? s1 >> (8 * k) : s0 >> (8 * (k - 4))) & 0xffu) << (8 * i);
+    }
+    return r;
+}
+
 }  // namespace sqemu
 
 typedef int sqemu_v4i __attribute__((ext_vector_type(4)));
@@ -365,6 +376,7 @@ inline sqemu_v16f mfma_f32_32x32x8f16(sqemu_v4h a, sqemu_v4h b, sqemu_v16f c) {
 #define __builtin_amdgcn_sched_barrier(m) ((void)(m))
 // v_exp_f32 (2^x): the host exp2f stands in for the device instruction
 #define __builtin_amdgcn_exp2f(x) ::exp2f((float)(x))
+#define __builtin_amdgcn_perm(a, b, s) ::sqemu::perm((a), (b), (s))
 #define __builtin_amdgcn_sdot4(a, b, c, cl) ::sqemu::sdot4((a), (b), (c), (cl))
 #define __builtin_amdgcn_mfma_i32_16x16x32_i8(a, b, c, x, y, z) ::sqemu::mfma_i32_16x16x32_i8((a), (b), (c))
 #define __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, x, y, z) ::sqemu::mfma_f32_16x16x4f32((a), (b), (c))
