@@ -22,8 +22,9 @@ HIP_FLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}",
              "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
              "-Wall", "-Wno-unused-function", "-Wno-unused-variable"]
 # Per-file additions.  The prefill matmul converts every MFMA result on the
-# VALU, so its results are placed straight in VGPRs (no AGPR copy-out).
-FILE_FLAGS = {"k_gemm.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"]}
+# VALU, so its results are placed straight in VGPRs (no AGPR copy-out); so does
+# the paged attention, for its softmax and the rescaling of its sums.
+FILE_FLAGS = {f: ["-mllvm", "-amdgpu-mfma-vgpr-form"] for f in ("k_gemm.hip", "k_paged.hip")}
 CXX_FLAGS = ["-x", "c++", "-O2", "-std=c++17", "-fPIC", "-Wall", "-Wno-unused-function",
              "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include"]
 

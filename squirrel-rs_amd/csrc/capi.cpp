@@ -599,6 +599,8 @@ int sq_sdpa_paged(sq_kv_plan* plan, size_t layer, const float* d_q, size_t q_str
     if (st) return finish(st);
     if (pv.rows == 0) return 0;
     if (!d_q || !d_out) return finish(set_error(SQ_ERR_ARG, "sdpa_paged: null argument"));
+    if ((size_t)pv.rows * n_heads > (size_t)INT32_MAX)
+        return finish(set_error(SQ_ERR_SHAPE, "sdpa_paged: ShapeMismatch (too many rows)"));
     size_t longest = 0;
     for (const KvSeq& s : plan->seqs) longest = std::max(longest, (size_t)s.past + s.n_new);
     // (a window that reaches over every sequence is none)

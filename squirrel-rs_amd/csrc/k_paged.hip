@@ -13,6 +13,7 @@ namespace sq {
 namespace {
 
 typedef float v4f __attribute__((ext_vector_type(4)));
+typedef float v2f __attribute__((ext_vector_type(2)));
 typedef _Float16 v2h __attribute__((ext_vector_type(2)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 
@@ -21,6 +22,20 @@ inline int check_launch(const char* what) {
     if (e != hipSuccess) return set_error(SQ_ERR_HIP, std::string(what) + ": " + hipGetErrorString(e));
     return 0;
 }
+
+// Division of x < 2^31 by a number that a launch knows: with m = ceil(2^32 / d)
+// floor(x m / 2^32) is the quotient or one more.  (The dozen divisions at a workgroup's
+// start cost 1.5 us of one token's 5.5 as the compiler makes them.)
+struct alignas(8) Div {
+    uint32_t d, m;  // (m = 0: d = 1)
+    Div() = default;
+    explicit Div(int n) : d((uint32_t)n), m((uint32_t)((((uint64_t)1 << 32) + d - 1) / d)) {}
+    __host__ __device__ int operator()(int x) const {
+        if (d == 1) return x;
+        const uint32_t q = (uint32_t)(((uint64_t)(uint32_t)x * m) >> 32);
+        return (int)(q * d > (uint32_t)x ? q - 1 : q);
+    }
+};
 
 // The query rows of one KV head of a sequence are its n_new * G (position,
 // head) pairs, row r = i * G + (head in the group).
@@ -44,14 +59,16 @@ __host__ __device__ inline Span tile_span(int pos_lo, int pos_hi, int window, in
 }
 
 // What a launch covers: the sequences with rows_lo <= n_new * G <= rows_hi,
-// their pages cut into parts of `chunk`.  The parts' sums stand in the
-// workspace at slot (table0 / chunk + sequence + part): a sequence has at
-// most pages / chunk + 1 parts, so slots do not overlap.
+// their pages cut into parts of `chunk` (the last one holds between a half and
+// one and a half of it).  The parts' sums stand in the workspace at slot (table0 / chunk + sequence + part): a sequence has
+// at most pages / chunk + 1 parts, so slots do not overlap.
 struct Cut {
-    int rows_lo, rows_hi, chunk, tiles, splits;
+    int rows_lo, rows_hi, chunk, tiles, splits, pad;
+    Div by_chunk, by_group, by_heads;  // chunk, heads / kv_heads, kv_heads
     float* ws;
+    __host__ __device__ int parts(int count) const { return count < chunk ? 1 : by_chunk(count + (chunk >> 1)); }
     __host__ __device__ size_t slot(const KvSeq& s, int seq, int part) const {
-        return (size_t)(s.table0 / chunk) + seq + part;
+        return (size_t)by_chunk(s.table0) + seq + part;
     }
 };
 
@@ -79,88 +96,213 @@ __device__ __forceinline__ float groups_sum(float v) {
     return v + __shfl_xor(v, 32, 64);
 }
 
+// E consecutive dimensions of one query row from `d`, rotated; false where one
+// is not finite.
+template <int E>
+__device__ __forceinline__ bool load_query(const float* q, bool vec, const double2* rope, int half, int d, float* x) {
+    if (vec) {
+#pragma unroll
+        for (int e = 0; e < E; e += 4) {
+            const float4 f = *(const float4*)(q + d + e);
+            x[e] = f.x, x[e + 1] = f.y, x[e + 2] = f.z, x[e + 3] = f.w;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; e++) x[e] = q[d + e];
+    }
+    bool ok = true;
+#pragma unroll
+    for (int e = 0; e < E; e++) ok = ok && fabsf(x[e]) < INFINITY;
+    if (rope && d / 2 < half) {
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+            const int j = (d + e) / 2;
+            const double2 cs = rope[min(j, half - 1)];
+            const double u = x[e], v = x[e + 1];
+            if (j < half) {
+                x[e] = (float)(u * cs.x - v * cs.y);
+                x[e + 1] = (float)(u * cs.y + v * cs.x);
+            }
+        }
+    }
+    return ok;
+}
+
+// The power of two that brings a row's largest magnitude to 2^13 .. 2^14, and what
+// turns products of the scaled row into scores.  A row that is not finite, or
+// leaves f32 by its rotation, has NaN scores (shift -1000: its halves are zeros).
+__device__ __forceinline__ int query_shift(float amax, float scale, float& cq) {
+    if (!(amax < INFINITY)) {
+        cq = NAN;
+        return -1000;
+    }
+    const int shift = min(140 - (int)((__builtin_bit_cast(uint32_t, amax) >> 23) & 255), 100);
+    cq = ldexpf(scale, -shift);
+    return shift;
+}
+__device__ __forceinline__ void halves(float x, int shift, _Float16& h, _Float16& lo) {
+    const float y = shift == -1000 ? 0.0f : ldexpf(x, shift);
+    h = (_Float16)y;
+    lo = (_Float16)(y - (float)h);
+}
+
 // Scores are formed transposed, K Q^T, so that a lane holds one query's
 // probabilities of sixteen positions, in the order of the stored values: they
 // are the second product's operand as they stand (V^T P^T), and its results,
 // dimensions of the same query, are scaled lane by lane.
 //
 // The cached integers are exact in f16.  A query's elements, scaled by a power
-// of two to at most 2^14, and a page's probabilities, times 2^14, are split into
+// of two to at most 2^14, and a page's probabilities, times 2^kBase, are split into
 // two f16 halves each (x = hi + lo to 2^-22 of x): two products on the matrix
 // pipe give what one in f32 would, four times as fast.
 //
-// PAGES: the four wavefronts take pages in turn for the same 16 R rows and meet in
+// A row's maximum follows its scores in steps: as long as they stay within
+// kHeadroom of it (in powers of two) nothing is rescaled, and the weights
+// stay below 2^(kBase + kHeadroom + 1) = 2^15, in f16's range with kBase bits
+// of room for the small ones.
+//
+// PAGES: the wavefronts take pages in turn for the same 16 R rows and meet in
 // LDS; otherwise each has its own 16 R rows and all walk the same pages.
-template <int HD, int R, bool PAGES>
-__global__ __launch_bounds__(256) void sdpa_paged_kernel(KvView kv, KvPlanView pl, PagedArgs a, Cut cut, float scale) {
-    constexpr int C = HD / 64, DT = HD / 16, TR = PAGES ? 16 * R : 64 * R;
-    __shared__ float s_o[PAGES ? 4 * 16 * R * (HD + 4) : 1];
-    __shared__ float s_m[PAGES ? 4 * 16 * R : 1], s_l[PAGES ? 4 * 16 * R : 1];
-    int b = blockIdx.x;
-    const int head = b % kv.kv_heads;
-    b /= kv.kv_heads;
-    const int part = b % cut.splits;
-    b /= cut.splits;
-    const int tile = b % cut.tiles, seq = b / cut.tiles;
+constexpr int kStat = 4;  // floats behind a part's sums: the maximum, the sum of weights, two unused
+constexpr float kBase = 8.0f, kHeadroom = 6.0f;
+constexpr float kSmall = 0x1p-8f;  // of the sums' unit: the scales of a page's values that need no other
+template <int HD, int R, int NW, bool PAGES>
+__global__ __launch_bounds__(NW * 64, PAGES ? (HD == 64 ? 3 : 2) : 2) void sdpa_paged_kernel(KvView kv, KvPlanView pl, PagedArgs a, Cut cut, float scale) {
+    constexpr int C = HD / 64, DT = HD / 16, TR = PAGES ? 16 * R : NW * 16 * R;
+    __shared__ __attribute__((aligned(16))) float s_o[PAGES ? NW * 16 * R * (HD + 4) : 1];
+    __shared__ __attribute__((aligned(16))) _Float16 s_q[2][PAGES ? 16 * R * HD : 8];
+    __shared__ float s_cq[PAGES ? 16 * R : 1];
+    __shared__ float s_m[PAGES ? NW * 16 * R : 1], s_l[PAGES ? NW * 16 * R : 1];
+    // (heads next to each other: with eight of them each is one XCD's, and a
+    // head's tiles share that XCD's L2; a sequence's last tiles, which see the most
+    // pages, first)
+    const int at = cut.by_heads(blockIdx.x), head = blockIdx.x - at * kv.kv_heads, tile = cut.tiles - 1 - at;
+    const int part = blockIdx.y, seq = blockIdx.z;
     const KvSeq s = pl.seqs[seq];
-    const int G = a.heads / kv.kv_heads, rows = s.n_new * G;
+    const int G = (int)cut.by_group.d, rows = s.n_new * G;
     if (rows < cut.rows_lo || rows > cut.rows_hi || tile * TR >= rows) return;
     const int row_end = min(rows, (tile + 1) * TR);
-    const Span span = tile_span(s.past + tile * TR / G, s.past + (row_end - 1) / G, a.window, a.sinks);
-    const int i_end = min(span.count, (part + 1) * cut.chunk);
-    if (part * cut.chunk >= i_end) return;
-    const bool whole = span.count <= cut.chunk;
+    const Span span = tile_span(s.past + cut.by_group(tile * TR), s.past + cut.by_group(row_end - 1), a.window, a.sinks);
+    const int parts = cut.parts(span.count);
+    if (part >= parts) return;
+    const int i_end = part == parts - 1 ? span.count : (part + 1) * cut.chunk;
+    const bool whole = parts == 1;
 
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, q16 = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, q16 = lane & 15, g = lane >> 4;
     const int row0 = tile * TR + (PAGES ? 0 : wave * 16 * R);  // the wavefront's first row
 
-    // queries: halves [chunk of 64][half of a lane's 16 dimensions]
+    // The bytes of one page in registers: keys, then values.  A page's keys are
+    // requested before the second product of the page before, its values
+    // behind it.
+    const int step = PAGES ? NW : 1;
+    int i = part * cut.chunk + (PAGES ? wave : 0);
+    uint4 kw[4][C], vw[DT];
+    float2 sc = make_float2(0.0f, 0.0f), sc_next = sc;
+    const uint4* kb = nullptr;
+    auto locate = [&](int i) {
+        const size_t cell = (size_t)pl.pages[s.table0 + span.page(i)] * kv.kv_heads + head;
+        sc_next = kv.scales[cell];
+        kb = (const uint4*)(kv.bytes + cell * 2 * kPage * HD) + lane;
+    };
+    auto load_keys = [&] {
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int c = 0; c < C; c++) kw[t][c] = kb[(t * C + c) * 64];
+    };
+    auto load_values = [&] {
+#pragma unroll
+        for (int d = 0; d < DT; d++) vw[d] = kb[(4 * C + d) * 64];
+    };
+    if (i < i_end) {
+        locate(i);
+        load_keys();
+        load_values();
+    }
+
+    // Queries: [chunk of 64][half of a lane's 16 dimensions].
     v8h qh[R][C][2], ql[R][C][2];
     float cq[R];
     int pos[R], w0[R];
+    const bool vec = (((uintptr_t)a.q | (a.q_stride * 4)) & 15) == 0;
+    auto query = [&](int r) {
+        const int i = cut.by_group(r);
+        return a.q + ((size_t)s.row0 + i) * a.q_stride + (size_t)(head * G + r - i * G) * HD;
+    };
+    auto rope = [&](int r) { return pl.rope ? pl.rope + ((size_t)s.row0 + cut.by_group(r)) * pl.half : nullptr; };
 #pragma unroll
-    for (int t = 0; t < R; t++) {
-        const int r = min(row0 + 16 * t + q16, rows - 1), i = r / G;
-        pos[t] = s.past + i;
-        w0[t] = a.window && a.window <= pos[t] ? pos[t] - a.window + 1 : 0;
-        const size_t row = (size_t)s.row0 + i;
-        const float* q = a.q + row * a.q_stride + (size_t)(head * G + r % G) * HD;
-        float x[C][16];
-        float amax = 0.0f;
-        bool ok = true;
+    for (int u = 0; u < R; u++) {
+        const int r = min(row0 + 16 * u + q16, rows - 1);
+        pos[u] = s.past + cut.by_group(r);
+        w0[u] = a.window && a.window <= pos[u] ? pos[u] - a.window + 1 : 0;
+    }
+    if constexpr (PAGES) {
+        // Once for the workgroup, HD / 16 consecutive dimensions a thread (16 lanes
+        // are a row), handed over in the operand's order.  (Every wavefront for
+        // itself: 64 lanes in as many cache lines for each load, 27.8 us instead of
+        // 32.8 for 48 chats.)
+        constexpr int E = HD / 16;
+        static_assert(256 * R <= NW * 64, "a thread has one piece of the rows");
+        if (threadIdx.x < 256 * R) {
+            const int u = threadIdx.x >> 8, e0 = (threadIdx.x & 15) * E, k = (threadIdx.x >> 4) & 15, r = row0 + 16 * u + k;
+            float x[E] = {};
+            float amax = 0.0f, c = 0.0f;
+            bool ok = true;
+            if (r < rows) {
+                ok = load_query<E>(query(r), vec, rope(r), pl.half, e0, x);
 #pragma unroll
-        for (int c = 0; c < C; c++)
+                for (int e = 0; e < E; e++) amax = fmaxf(amax, fabsf(x[e]));
+            }
+            const int shift = query_shift(sq_row_max(ok ? amax : INFINITY), scale, c);
+            if ((threadIdx.x & 15) == 0) s_cq[u * 16 + k] = c;
+            // dimension d: chunk d / 64, lane group (d / 16) % 4, half (d / 8) % 2
+            const int at = (((u * C + (e0 >> 6)) * 2 + ((e0 >> 3) & 1)) * 64 + ((e0 >> 4) & 3) * 16 + k) * 8 + (e0 & 7);
 #pragma unroll
-            for (int e = 0; e < 16; e += 2) {
-                const int d = 64 * c + 16 * g + e;
-                float u = q[d], v = q[d + 1];
-                ok = ok && fabsf(u) < INFINITY && fabsf(v) < INFINITY;
-                if (pl.rope && d / 2 < pl.half) {
-                    const double2 cs = pl.rope[row * pl.half + d / 2];
-                    const double p = (double)u * cs.x - (double)v * cs.y;
-                    v = (float)((double)u * cs.y + (double)v * cs.x);
-                    u = (float)p;
+            for (int e = 0; e < E; e++) halves(x[e], shift, s_q[0][at + e], s_q[1][at + e]);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < R; u++) {
+            cq[u] = s_cq[u * 16 + q16];
+#pragma unroll
+            for (int c = 0; c < C; c++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    qh[u][c][h] = *(const v8h*)&s_q[0][(((u * C + c) * 2 + h) * 64 + lane) * 8];
+                    ql[u][c][h] = *(const v8h*)&s_q[1][(((u * C + c) * 2 + h) * 64 + lane) * 8];
                 }
-                x[c][e] = u, x[c][e + 1] = v;
-                amax = fmaxf(amax, fmaxf(fabsf(u), fabsf(v)));
-            }
-        // (a row that is not finite, or leaves f32 by its rotation: NaN scores for it alone)
-        amax = groups_max(ok ? amax : INFINITY);
-        const int shift = amax < INFINITY ? min(13 - (int)((__builtin_bit_cast(uint32_t, amax) >> 23) & 255) + 127, 100) : 0;
-        cq[t] = amax < INFINITY ? ldexpf(scale, -shift) : NAN;
+        }
+    } else {
 #pragma unroll
-        for (int c = 0; c < C; c++)
+        for (int u = 0; u < R; u++) {
+            const int r = min(row0 + 16 * u + q16, rows - 1);
+            float x[C][16];
+            float amax = 0.0f;
+            bool ok = true;
 #pragma unroll
-            for (int e = 0; e < 16; e++) {
-                const float y = amax < INFINITY ? ldexpf(x[c][e], shift) : 0.0f;
-                const _Float16 h = (_Float16)y;
-                qh[t][c][e / 8][e % 8] = h;
-                ql[t][c][e / 8][e % 8] = (_Float16)(y - (float)h);
+            for (int c = 0; c < C; c++) {
+                ok = load_query<16>(query(r), vec, rope(r), pl.half, 64 * c + 16 * g, x[c]) && ok;
+#pragma unroll
+                for (int e = 0; e < 16; e++) amax = fmaxf(amax, fabsf(x[c][e]));
             }
+            const int shift = query_shift(groups_max(ok ? amax : INFINITY), scale, cq[u]);
+#pragma unroll
+            for (int c = 0; c < C; c++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    _Float16 h, lo;
+                    halves(x[c][e], shift, h, lo);
+                    qh[u][c][e / 8][e % 8] = h, ql[u][c][e / 8][e % 8] = lo;
+                }
+        }
     }
 
+    // (-1 that the compiler does not know to be: p - h then takes the f16 half as it
+    // is, where it would convert it to f32 first)
+    float minus = -1.0f;
+    asm volatile("" : "+v"(minus));
     v4f o[R][DT];
-    float m[R], l[R];
+    float m[R], l[R], vref = 0.0f, vtop = 0.0f;
 #pragma unroll
     for (int t = 0; t < R; t++) {
         m[t] = -INFINITY, l[t] = 0.0f;
@@ -168,22 +310,12 @@ __global__ __launch_bounds__(256) void sdpa_paged_kernel(KvView kv, KvPlanView p
         for (int d = 0; d < DT; d++) o[t][d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
     }
     // rows between the tile's first and last position see a page whole where both do
-    const int pos_lo = s.past + row0 / G, pos_hi = s.past + (min(rows, row0 + 16 * R) - 1) / G;
+    const int pos_lo = s.past + cut.by_group(row0), pos_hi = s.past + cut.by_group(min(rows, row0 + 16 * R) - 1);
     const int w0_hi = a.window && a.window <= pos_hi ? pos_hi - a.window + 1 : 0;
 
-    const int step = PAGES ? 4 : 1;
-    for (int i = part * cut.chunk + (PAGES ? wave : 0); i < i_end; i += step) {
+    for (; i < i_end; i += step) {
         const int page = span.page(i);
-        const size_t cell = (size_t)pl.pages[s.table0 + page] * kv.kv_heads + head;
-        const float2 sc = kv.scales[cell];
-        const uint4* kb = (const uint4*)(kv.bytes + cell * 2 * kPage * HD) + lane;
-        uint4 kw[4][C], vw[DT];
-#pragma unroll
-        for (int t = 0; t < 4; t++)
-#pragma unroll
-            for (int c = 0; c < C; c++) kw[t][c] = kb[(t * C + c) * 64];
-#pragma unroll
-        for (int d = 0; d < DT; d++) vw[d] = kb[(4 * C + d) * 64];
+        sc = sc_next;
         // scores [tile of 16 positions][position 4 g + r]
         v4f x[R][4];
 #pragma unroll
@@ -203,94 +335,141 @@ __global__ __launch_bounds__(256) void sdpa_paged_kernel(KvView kv, KvPlanView p
             }
         }
         const bool full = (page + 1) * kPage - 1 <= pos_lo && (page * kPage >= w0_hi || (page + 1) * kPage <= a.sinks);
+        // The sums stand in units of vref, near the scale of the page's values; a
+        // page's weights carry the rest of it, so that the matrix pipe adds to the
+        // sums in place.  (The unit goes no further than 2^-64 below the largest
+        // so far: the sums stay in range, and what that costs is 2^-70 of those
+        // values.  A page of zeros adds nothing in any unit.)
+        if (sc.y > 0.0f && !(sc.y <= 2.0f * vref && sc.y >= kSmall * vref)) {
+            vtop = fmaxf(vtop, sc.y);
+            const float to = fmaxf(sc.y, 0x1p-64f * vtop), f = vref > 0.0f ? vref / to : 0.0f;
+#pragma unroll
+            for (int u = 0; u < R; u++)
+#pragma unroll
+                for (int d = 0; d < DT; d++) o[u][d] *= f;
+            vref = to;
+        }
+        const float lr = sc.y > 0.0f ? __builtin_amdgcn_logf(sc.y / vref) : 0.0f, back = __builtin_amdgcn_exp2f(-lr);
         v8h ph[R][2], plo[R][2];
-        float alpha[R];
 #pragma unroll
         for (int u = 0; u < R; u++) {
-            const float cs = cq[u] * sc.x;
+            float cs = cq[u] * sc.x;
+            if (!full) {
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const int at = page * kPage + 16 * t + 4 * g + r;
+                        const bool hidden = (at > pos[u]) | ((at < w0[u]) & (at >= a.sinks));
+                        x[u][t][r] = hidden ? -INFINITY : x[u][t][r] * cs;
+                    }
+                cs = 1.0f;
+            }
             float mx = -INFINITY;
 #pragma unroll
             for (int t = 0; t < 4; t++)
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    float y = x[u][t][r] * cs;
-                    if (!full) {
-                        const int at = page * kPage + 16 * t + 4 * g + r;
-                        if (at > pos[u] || (at < w0[u] && at >= a.sinks)) y = -INFINITY;
-                    }
-                    x[u][t][r] = y;
-                    mx = fmaxf(mx, y);
-                }
-            const float mn = fmaxf(m[u], groups_max(mx));
-            const float base = mn == -INFINITY ? 0.0f : mn;
-            alpha[u] = __builtin_amdgcn_exp2f(m[u] - base);
-            m[u] = mn;
+                for (int r = 0; r < 4; r++) mx = fmaxf(mx, x[u][t][r]);
+            mx = groups_max(mx * cs);
+            if (__any(mx > m[u] + kHeadroom)) {
+                const float mn = fmaxf(m[u], mx);
+                const float alpha = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[u] - mn);
+                m[u] = mn;
+                l[u] *= alpha;
+#pragma unroll
+                for (int d = 0; d < DT; d++) o[u][d] *= alpha;
+            }
+            const float off = kBase - (m[u] == -INFINITY ? 0.0f : m[u]) + lr;
             float sum = 0.0f;
 #pragma unroll
             for (int r = 0; r < 4; r++)
 #pragma unroll
-                for (int t = 0; t < 4; t++) {
-                    const float p = __builtin_amdgcn_exp2f(x[u][t][r] - base + 14.0f);
-                    sum += p;
-                    const _Float16 h = (_Float16)p;
+                for (int t = 0; t < 4; t += 2) {
+                    const v2f p = {__builtin_amdgcn_exp2f(fmaf(x[u][t][r], cs, off)),
+                                   __builtin_amdgcn_exp2f(fmaf(x[u][t + 1][r], cs, off))};
+                    sum += p[0] + p[1];
+                    const v2h h = __builtin_convertvector(p, v2h);
+                    const v2f rest = {fmaf((float)h[0], minus, p[0]), fmaf((float)h[1], minus, p[1])};
+                    const v2h w = __builtin_convertvector(rest, v2h);
                     const int j = 4 * r + t;
-                    ph[u][j / 8][j % 8] = h;
-                    plo[u][j / 8][j % 8] = (_Float16)(p - (float)h);
+                    ph[u][j / 8][j % 8] = h[0], ph[u][j / 8][j % 8 + 1] = h[1];
+                    plo[u][j / 8][j % 8] = w[0], plo[u][j / 8][j % 8 + 1] = w[1];
                 }
-            l[u] = l[u] * alpha[u] + sum;
+            l[u] += sum * back;
         }
+        const bool more = i + step < i_end;
+        if (more) {
+            locate(i + step);
+            load_keys();
+        }
+        auto weigh = [&](int u, v8h v0, v8h v1, v4f y) {
+            y = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, plo[u][0], y, 0, 0, 0);
+            y = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, plo[u][1], y, 0, 0, 0);
+            y = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, ph[u][0], y, 0, 0, 0);
+            return __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, ph[u][1], y, 0, 0, 0);
+        };
 #pragma unroll
         for (int d = 0; d < DT; d++) {
             const v8h v0 = unpack8(vw[d].x, vw[d].y), v1 = unpack8(vw[d].z, vw[d].w);
 #pragma unroll
-            for (int u = 0; u < R; u++) {
-                v4f y = {0.0f, 0.0f, 0.0f, 0.0f};
-                y = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, plo[u][0], y, 0, 0, 0);
-                y = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, plo[u][1], y, 0, 0, 0);
-                y = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, ph[u][0], y, 0, 0, 0);
-                y = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, ph[u][1], y, 0, 0, 0);
-#pragma unroll
-                for (int r = 0; r < 4; r++) o[u][d][r] = o[u][d][r] * alpha[u] + y[r] * sc.y;
-            }
+            for (int u = 0; u < R; u++) o[u][d] = weigh(u, v0, v1, o[u][d]);
         }
+        if (more) load_values();
     }
+#pragma unroll
+    for (int u = 0; u < R; u++)
+#pragma unroll
+        for (int d = 0; d < DT; d++) o[u][d] *= vref;
 #pragma unroll
     for (int u = 0; u < R; u++) l[u] = groups_sum(l[u]);
 
-    // where row r's sums go: its output, or its part of the workspace
-    auto emit = [&](int r, int d, float v, float mm, float ll) {
+    // where four of row r's sums go: its output, or its part of the workspace
+    const bool vec_out = (((uintptr_t)a.out | (a.out_stride * 4)) & 15) == 0;
+    auto emit = [&](int r, int d, v4f v, float mm, float ll) {
         if (whole) {
-            a.out[((size_t)s.row0 + r / G) * a.out_stride + (size_t)(head * G + r % G) * HD + d] = v / ll;
+            const int i = cut.by_group(r);
+            float* out = a.out + ((size_t)s.row0 + i) * a.out_stride + (size_t)(head * G + r - i * G) * HD + d;
+            v *= 1.0f / ll;
+            if (vec_out) {
+                *(v4f*)out = v;
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; k++) out[k] = v[k];
+            }
         } else {
             const size_t at = (cut.slot(s, seq, part) * kv.kv_heads + head) * cut.rows_hi + r;
-            float* w = cut.ws + at * (HD + 2);
-            w[d] = v;
-            if (d == 0) w[HD] = mm, w[HD + 1] = ll;
+            float* w = cut.ws + at * (HD + kStat);
+            *(v4f*)(w + d) = v;
+            if (d == 0) *(v2f*)(w + HD) = v2f{mm, ll};
         }
     };
     if constexpr (PAGES) {
+        // (a wavefront that saw nothing has no weight; NaN scores keep their NaN)
 #pragma unroll
         for (int u = 0; u < R; u++) {
-            const int r = wave * 16 * R + 16 * u + q16;
-            if (g == 0) s_m[r] = m[u], s_l[r] = l[u];
+            const int r = 16 * u + q16, k = wave * 16 * R + r;
+            if (row0 + r < rows) {
+                if (g == 0) s_m[k] = m[u], s_l[k] = l[u];
 #pragma unroll
-            for (int d = 0; d < DT; d++) *(v4f*)&s_o[r * (HD + 4) + 16 * d + 4 * g] = o[u][d];
+                for (int d = 0; d < DT; d++) *(v4f*)&s_o[k * (HD + 4) + 16 * d + 4 * g] = o[u][d];
+            }
         }
         __syncthreads();
-        for (int e = threadIdx.x; e < 16 * R * HD; e += 256) {
-            const int r = e / HD, d = e % HD;
+        for (int e = threadIdx.x; e < 16 * R * (HD / 4); e += NW * 64) {
+            const int r = e / (HD / 4), d = e % (HD / 4) * 4;
             if (row0 + r >= rows) break;
-            float mm = -INFINITY, ll = 0.0f, v = 0.0f;
+            float mm = -INFINITY, ll = 0.0f;
+            v4f v = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int w = 0; w < 4; w++) mm = fmaxf(mm, s_m[w * 16 * R + r]);
+            for (int w = 0; w < NW; w++) mm = fmaxf(mm, s_m[w * 16 * R + r]);
+            const float base = mm == -INFINITY ? 0.0f : mm;
 #pragma unroll
-            for (int w = 0; w < 4; w++) {
+            for (int w = 0; w < NW; w++) {
                 const int k = w * 16 * R + r;
-                // (no page, or none visible: nothing; NaN scores keep their NaN)
-                const float f = s_m[k] == -INFINITY && s_l[k] == 0.0f ? 0.0f
-                                : __builtin_amdgcn_exp2f((s_m[k] == -INFINITY ? 0.0f : s_m[k]) - (mm == -INFINITY ? 0.0f : mm));
-                ll += s_l[k] * f;
-                v += s_o[k * (HD + 4) + d] * f;
+                const float m1 = s_m[k], l1 = s_l[k];
+                const float f = __builtin_amdgcn_exp2f((m1 == -INFINITY && l1 != 0.0f ? 0.0f : m1) - base);
+                ll += l1 * f;
+                v += *(const v4f*)&s_o[k * (HD + 4) + d] * f;
             }
             emit(row0 + r, d, v, mm, ll);
         }
@@ -300,62 +479,75 @@ __global__ __launch_bounds__(256) void sdpa_paged_kernel(KvView kv, KvPlanView p
             const int r = row0 + 16 * u + q16;
             if (r >= rows) continue;
 #pragma unroll
-            for (int d = 0; d < DT; d++)
-#pragma unroll
-                for (int k = 0; k < 4; k++) emit(r, 16 * d + 4 * g + k, o[u][d][k], m[u], l[u]);
+            for (int d = 0; d < DT; d++) emit(r, 16 * d + 4 * g, o[u][d], m[u], l[u]);
         }
     }
 }
 
-// The parts of the rows whose pages were cut: one workgroup per (sequence,
-// KV head, row), a wavefront per quarter of the parts.
+// The parts of the rows whose pages were cut: one workgroup per (sequence, KV
+// head, row).  A wavefront's lanes find the factors of 64 parts, then it adds
+// every fourth part, eight in flight at a time.
 template <int HD>
 __global__ __launch_bounds__(256) void sdpa_merge_kernel(KvView kv, KvPlanView pl, PagedArgs a, Cut cut, int tile_rows) {
-    __shared__ float s_o[4][HD], s_m[4], s_l[4];
-    const int seq = blockIdx.y, head = blockIdx.x % kv.kv_heads, r = blockIdx.x / kv.kv_heads;
+    constexpr int C = HD / 64, IN = 8;
+    __shared__ float s_o[4][HD];
+    const int seq = blockIdx.y, r = cut.by_heads(blockIdx.x), head = blockIdx.x - r * kv.kv_heads;
     const KvSeq s = pl.seqs[seq];
-    const int G = a.heads / kv.kv_heads, rows = s.n_new * G;
+    const int G = (int)cut.by_group.d, rows = s.n_new * G;
     if (rows < cut.rows_lo || rows > cut.rows_hi || r >= rows) return;
     const int tile = r / tile_rows, row_end = min(rows, (tile + 1) * tile_rows);
-    const Span span = tile_span(s.past + tile * tile_rows / G, s.past + (row_end - 1) / G, a.window, a.sinks);
-    if (span.count <= cut.chunk) return;
-    const int parts = (span.count + cut.chunk - 1) / cut.chunk;
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const size_t stride = (size_t)kv.kv_heads * cut.rows_hi * (HD + 2);
-    const float* w = cut.ws + ((cut.slot(s, seq, 0) * kv.kv_heads + head) * cut.rows_hi + r) * (HD + 2);
-    float m = -INFINITY, l = 0.0f, o[HD / 64] = {};
-    auto fold = [](float& m, float& l, float* o, float m1, float l1, const float* o1) {
-        const float mn = fmaxf(m, m1), base = mn == -INFINITY ? 0.0f : mn;
-        const float f = __builtin_amdgcn_exp2f(m - base);
-        const float f1 = m1 == -INFINITY && l1 == 0.0f ? 0.0f
-                         : __builtin_amdgcn_exp2f((m1 == -INFINITY ? 0.0f : m1) - base);
-        m = mn;
-        l = l * f + l1 * f1;
-        for (int c = 0; c < HD / 64; c++) o[c] = o[c] * f + o1[c] * f1;
-    };
-    for (int i = wave; i < parts; i += 4) {
-        const float* p = w + (size_t)i * stride;
-        float o1[HD / 64];
-        for (int c = 0; c < HD / 64; c++) o1[c] = p[64 * c + lane];
-        fold(m, l, o, p[HD], p[HD + 1], o1);
+    const Span span = tile_span(s.past + cut.by_group(tile * tile_rows), s.past + cut.by_group(row_end - 1), a.window, a.sinks);
+    const int parts = cut.parts(span.count);
+    if (parts == 1) return;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    const size_t stride = (size_t)kv.kv_heads * cut.rows_hi * (HD + kStat);
+    const float* w = cut.ws + ((cut.slot(s, seq, 0) * kv.kv_heads + head) * cut.rows_hi + r) * (HD + kStat);
+    float mm = -INFINITY, ll = 0.0f, o[C] = {};
+    for (int i = lane; i < parts; i += 64) mm = fmaxf(mm, w[i * stride + HD]);
+    mm = sq_wave_max(mm);
+    for (int i0 = 0; i0 < parts; i0 += 64) {
+        float f = 0.0f;
+        if (i0 + lane < parts) {
+            const float m1 = w[(i0 + lane) * stride + HD], l1 = w[(i0 + lane) * stride + HD + 1];
+            // (a part that saw nothing adds nothing; NaN scores keep their NaN)
+            f = __builtin_amdgcn_exp2f((m1 == -INFINITY && l1 != 0.0f ? 0.0f : m1) - (mm == -INFINITY ? 0.0f : mm));
+            ll += l1 * f;
+        }
+        const int n = min(parts - i0, 64);
+        for (int k = wave; k < n; k += 4 * IN) {
+            float v[IN][C];
+#pragma unroll
+            for (int j = 0; j < IN; j++)
+#pragma unroll
+                for (int c = 0; c < C; c++) v[j][c] = w[(i0 + min(k + 4 * j, n - 1)) * stride + 64 * c + lane];
+#pragma unroll
+            for (int j = 0; j < IN; j++) {
+                const float fj = __builtin_bit_cast(
+                    float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), min(k + 4 * j, 63)));
+                if (k + 4 * j < n)
+#pragma unroll
+                    for (int c = 0; c < C; c++) o[c] += v[j][c] * fj;
+            }
+        }
     }
-    for (int c = 0; c < HD / 64; c++) s_o[wave][64 * c + lane] = o[c];
-    if (lane == 0) s_m[wave] = m, s_l[wave] = l;
+    ll = sq_wave_sum(ll);
+#pragma unroll
+    for (int c = 0; c < C; c++) s_o[wave][64 * c + lane] = o[c];
     __syncthreads();
     if (wave) return;
-    for (int k = 1; k < 4; k++) {
-        float o1[HD / 64];
-        for (int c = 0; c < HD / 64; c++) o1[c] = s_o[k][64 * c + lane];
-        fold(m, l, o, s_m[k], s_l[k], o1);
+    const int i = cut.by_group(r);
+    float* out = a.out + ((size_t)s.row0 + i) * a.out_stride + (size_t)(head * G + r - i * G) * HD;
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+        const int d = 64 * c + lane;
+        out[d] = ((s_o[0][d] + s_o[1][d]) + (s_o[2][d] + s_o[3][d])) / ll;
     }
-    float* out = a.out + ((size_t)s.row0 + r / G) * a.out_stride + (size_t)(head * G + r % G) * HD;
-    for (int c = 0; c < HD / 64; c++) out[64 * c + lane] = o[c] / l;
 }
 
 // Sequences of few rows: wavefronts over pages, tiles of 16 rows; of more: wavefronts over
-// rows, tiles of 128.
-constexpr int kFewRows = 64, kTileFew = 16, kTileMany = 128;
-constexpr int kTarget = 1024;  // workgroups that a launch is cut into
+// rows, tiles of 128 (of 64 with 128 dimensions, whose sums take the registers of two).
+constexpr int kFewWaves = 4, kFewRows = 64, kTileFew = 16, kTileMany = 128;
+constexpr int kTarget = 512, kTargetMany = 512;  // workgroups that a launch is cut into
 
 struct Launch {
     Cut cut;
@@ -363,9 +555,11 @@ struct Launch {
     bool any;
 };
 Launch plan_launch(const std::vector<KvSeq>& seqs, const KvView& kv, const PagedArgs& a, bool many) {
-    const int G = a.heads / kv.kv_heads, tile = many ? kTileMany : kTileFew;
+    const int G = a.heads / kv.kv_heads, tile = !many ? kTileFew : kv.head_dim == 64 ? kTileMany : kTileMany / 2;
     Launch r{};
     r.cut.rows_lo = many ? kFewRows + 1 : 1;
+    r.cut.by_group = Div(G);
+    r.cut.by_heads = Div(kv.kv_heads);
     long long work = 0, groups = 0, pages = 0;
     int longest = 0;
     for (const KvSeq& s : seqs) {
@@ -387,30 +581,34 @@ Launch plan_launch(const std::vector<KvSeq>& seqs, const KvView& kv, const Paged
     groups *= kv.kv_heads;
     // pages of a part: as many workgroups as the card takes at a time, unless
     // the tiles alone are
-    const int least = many ? 1 : 4;
-    long long chunk = groups >= kTarget ? longest : std::max<long long>(least, (work + kTarget - 1) / kTarget);
+    const int least = many ? 1 : 4 * kFewWaves;
+    const int target = many ? kTargetMany : kTarget;
+    long long chunk = std::max<long long>(least, (work + target - 1) / target);
+    if (many && groups >= target / 2) chunk = 2ll * longest;
     for (;; chunk *= 2) {
-        r.cut.chunk = (int)std::min<long long>(chunk, std::max(longest, 1));
-        r.cut.splits = (longest + r.cut.chunk - 1) / std::max(r.cut.chunk, 1);
+        r.cut.chunk = (int)std::min<long long>(chunk, 2ll * longest + 1);
+        r.cut.by_chunk = Div(r.cut.chunk);
+        r.cut.splits = r.cut.parts(longest);
         r.floats = r.cut.splits < 2 ? 0
                                     : (size_t)(pages / r.cut.chunk + seqs.size() + 1) * kv.kv_heads * r.cut.rows_hi *
-                                          (kv.head_dim + 2);
+                                          (kv.head_dim + kStat);
         if (r.floats <= ((size_t)64 << 20)) break;  // 256 MB
     }
     return r;
 }
 
-template <int HD, int R, bool PAGES>
+template <int HD, int R, int NW, bool PAGES>
 int launch_one(hipStream_t s, const Launch& l, const KvView& kv, const KvPlanView& p, const PagedArgs& a) {
     const float scale = 1.4426950408889634f / sqrtf((float)HD);  // scores in units of log 2
-    const size_t grid = (size_t)p.n_seqs * l.cut.tiles * l.cut.splits * kv.kv_heads;
+    const size_t grid = (size_t)l.cut.tiles * kv.kv_heads;
     const size_t merge = (size_t)l.cut.rows_hi * kv.kv_heads;
     if (grid > (size_t)INT32_MAX || merge > (size_t)INT32_MAX)
         return set_error(SQ_ERR_SHAPE, "sdpa_paged: ShapeMismatch (too many rows)");
-    hipLaunchKernelGGL((sdpa_paged_kernel<HD, R, PAGES>), dim3((unsigned)grid), dim3(256), 0, s, kv, p, a, l.cut, scale);
+    hipLaunchKernelGGL((sdpa_paged_kernel<HD, R, NW, PAGES>), dim3((unsigned)grid, l.cut.splits, p.n_seqs), dim3(NW * 64), 0, s, kv, p, a,
+                       l.cut, scale);
     if (l.cut.splits > 1)
         hipLaunchKernelGGL((sdpa_merge_kernel<HD>), dim3((unsigned)merge, p.n_seqs), dim3(256), 0, s, kv, p, a, l.cut,
-                           PAGES ? kTileFew : kTileMany);
+                           PAGES ? 16 * R : NW * 16 * R);
     return check_launch("sdpa_paged");
 }
 
@@ -428,9 +626,9 @@ int launch_sdpa_paged(hipStream_t s, const std::vector<KvSeq>& seqs, const KvVie
         l.cut.ws = ws;
         int st;
         if (kv.head_dim == 64)
-            st = many ? launch_one<64, 2, false>(s, l, kv, p, a) : launch_one<64, 1, true>(s, l, kv, p, a);
+            st = many ? launch_one<64, 2, 4, false>(s, l, kv, p, a) : launch_one<64, 1, kFewWaves, true>(s, l, kv, p, a);
         else
-            st = many ? launch_one<128, 2, false>(s, l, kv, p, a) : launch_one<128, 1, true>(s, l, kv, p, a);
+            st = many ? launch_one<128, 1, 4, false>(s, l, kv, p, a) : launch_one<128, 1, kFewWaves, true>(s, l, kv, p, a);
         if (st) return st;
     }
     return 0;

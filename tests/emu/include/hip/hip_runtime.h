@@ -193,6 +193,14 @@ inline int sdot4(int a, int b, int c, bool clamp) {
     return s;
 }
 
+// Whether any live lane's predicate holds.
+inline int any(bool p) {
+    const uint64_t* all = wave_exchange(p ? 1 : 0, 0x5000);
+    for (int l = 0; l < 64; l++)
+        if (all[l]) return 1;
+    return 0;
+}
+
 // v_perm_b32: byte i of the result is byte sel_i of {s1 (0-3), s0 (4-7)}.
 inline unsigned perm(unsigned s0, unsigned s1, unsigned sel) {
     unsigned r = 0;
@@ -376,6 +384,8 @@ inline sqemu_v16f mfma_f32_32x32x8f16(sqemu_v4h a, sqemu_v4h b, sqemu_v16f c) {
 #define __builtin_amdgcn_sched_barrier(m) ((void)(m))
 // v_exp_f32 (2^x): the host exp2f stands in for the device instruction
 #define __builtin_amdgcn_exp2f(x) ::exp2f((float)(x))
+#define __builtin_amdgcn_logf(x) ::log2f((float)(x))
+#define __any(p) ::sqemu::any((p) != 0)
 #define __builtin_amdgcn_perm(a, b, s) ::sqemu::perm((a), (b), (s))
 #define __builtin_amdgcn_sdot4(a, b, c, cl) ::sqemu::sdot4((a), (b), (c), (cl))
 #define __builtin_amdgcn_mfma_i32_16x16x32_i8(a, b, c, x, y, z) ::sqemu::mfma_i32_16x16x32_i8((a), (b), (c))
