@@ -633,15 +633,11 @@ int sq_verify_draft(const float* d_target, size_t target_stride, const float* d_
         return set_error(SQ_ERR_SHAPE, "verify_draft: ShapeMismatch (rows shorter than the vocabulary)");
     if (drafts && !d_tokens) return set_error(SQ_ERR_ARG, "verify_draft: null argument");
     const bool with_draft = d_draft && temperature > 0.0f;
-    Tmp res, ws;
+    PinnedTmp res;  // (the kernels write the results where the host reads them)
+    Tmp ws;
     int st;
     if ((st = res.alloc(n_seqs * sizeof(VerifyResult)))) return st;
-    std::vector<VerifyResult> host;
-    try {
-        host.resize(n_seqs);
-    } catch (const std::bad_alloc&) {
-        return set_error(SQ_ERR_ARG, "verify_draft: out of host memory");
-    }
+    const VerifyResult* host = (const VerifyResult*)res.p;
     // batches of sequences whose counts fit a launch's arguments; the
     // workspace of one serves the next (the null stream orders them)
     size_t t0 = 0, d0 = 0;
@@ -677,7 +673,6 @@ int sq_verify_draft(const float* d_target, size_t target_stride, const float* d_
         d0 += n_rows;
     }
     if ((st = finish(0))) return st;
-    SQ_HIP_CHECK(hipMemcpy(host.data(), res.p, n_seqs * sizeof(VerifyResult), hipMemcpyDeviceToHost));
     for (size_t i = 0; i < n_seqs; i++) {
         if (host[i].bad == 1)
             return set_error(SQ_ERR_ARG, "verify_draft: logits of sequence " + std::to_string(i) +

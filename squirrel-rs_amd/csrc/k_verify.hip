@@ -16,9 +16,10 @@
 namespace sq {
 namespace {
 
-constexpr int kBlock = 256;
-constexpr int kPer = 16;                    // logits of one thread
-constexpr int kChunk = kBlock * kPer;       // logits of one workgroup
+constexpr int kBlock = 512;
+constexpr int kPer = 8;                // logits of one thread, next to each other
+constexpr int kChunk = kBlock * kPer;  // logits of one workgroup
+constexpr int kWaves = kBlock / 64;
 
 inline int check_launch(const char* what) {
     hipError_t e = hipGetLastError();
@@ -26,89 +27,130 @@ inline int check_launch(const char* what) {
     return 0;
 }
 
-// A row's part: its maximum, the sum of 2^((l - max) inv_t) and the last index
-// of the maximum.  sum < 0: a value that is NaN or +inf is among them.
+// A chunk of a row: its maximum, the sum of 2^((l - max) inv_t) over it and the
+// last index of the maximum.  max = +inf: a value that is NaN or +inf is in it.
 struct Part {
     double sum;
     float max;
     uint32_t at;
 };
 
-// 2^x, x <= 0, to about 1e-14: Taylor's polynomial of 2^r on |r| <= 1/2.
-__device__ __forceinline__ double exp2_64(double x) {
-    if (x < -1060.0) return 0.0;  // (also -inf)
-    const double n = rint(x), r = (x - n) * 0.69314718055994530942;
-    double p = 1.0 / 6227020800.0;
-    p = fma(p, r, 1.0 / 479001600.0);
-    p = fma(p, r, 1.0 / 39916800.0);
-    p = fma(p, r, 1.0 / 3628800.0);
-    p = fma(p, r, 1.0 / 362880.0);
-    p = fma(p, r, 1.0 / 40320.0);
-    p = fma(p, r, 1.0 / 5040.0);
-    p = fma(p, r, 1.0 / 720.0);
-    p = fma(p, r, 1.0 / 120.0);
-    p = fma(p, r, 1.0 / 24.0);
-    p = fma(p, r, 1.0 / 6.0);
-    p = fma(p, r, 0.5);
-    p = fma(p, r, 1.0);
+// 2^((l - m) inv_t) for l <= m to 1.1e-12 of itself: 2^n times the polynomial
+// that meets 2^r at nine Chebyshev points of |r| <= 1/2.
+__device__ __forceinline__ double weight(float l, float m, double inv_t) {
+    const double x = fmax(((double)l - (double)m) * inv_t, -1100.0);  // (2^-1100 is 0; also for -inf)
+    const double n = rint(x), r = x - n;
+    double p = 1.3255224884796412e-06;
+    p = fma(p, r, 1.5310079402334074e-05);
+    p = fma(p, r, 0.00015403455852418322);
+    p = fma(p, r, 0.0013333450568000249);
+    p = fma(p, r, 0.009618129159402623);
+    p = fma(p, r, 0.055504109412059334);
+    p = fma(p, r, 0.2402265069581299);
+    p = fma(p, r, 0.6931471805459335);
     p = fma(p, r, 1.0);
     return ldexp(p, (int)n);
 }
 
-__device__ __forceinline__ double weight(float l, float m, double inv_t) {
-    return exp2_64(((double)l - (double)m) * inv_t);
+__device__ __forceinline__ double wave_sum64(double v) {
+#pragma unroll
+    for (int m = 1; m < 64; m *= 2) v += __shfl_xor(v, m, 64);
+    return v;
 }
 
-__device__ __forceinline__ void merge(Part& a, const Part& b, double inv_t) {
-    if (a.sum < 0.0 || b.sum < 0.0) {
-        a.sum = -1.0;
-        return;
+// Sums up to and including each lane's.
+__device__ __forceinline__ double wave_scan64(double v) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int k = 1; k < 64; k *= 2) {
+        const double up = __shfl_up(v, k, 64);
+        v += lane >= k ? up : 0.0;
     }
-    if (b.max > a.max || (b.max == a.max && b.at > a.at)) a.at = b.at;
-    const float m = fmaxf(a.max, b.max);
-    if (m != -INFINITY && inv_t > 0.0) a.sum = a.sum * weight(a.max, m, inv_t) + b.sum * weight(b.max, m, inv_t);
-    a.max = m;
+    return v;
 }
 
-__device__ __forceinline__ Part shuffled(const Part& p, int mask) {
-    return Part{__shfl_xor(p.sum, mask, 64), __shfl_xor(p.max, mask, 64), __shfl_xor(p.at, mask, 64)};
+// kPer logits from `i` on, -inf past the row.
+__device__ __forceinline__ void load_logits(const float* row, int i, int vocab, bool vec, float* x) {
+    if (vec && i + kPer <= vocab) {
+#pragma unroll
+        for (int e = 0; e < kPer; e += 4) {
+            const float4 f = *(const float4*)(row + i + e);
+            x[e] = f.x, x[e + 1] = f.y, x[e + 2] = f.z, x[e + 3] = f.w;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < kPer; e++) x[e] = i + e < vocab ? row[i + e] : -INFINITY;
+    }
 }
+__device__ __forceinline__ bool aligned(const float* row) { return ((uintptr_t)row & 15) == 0; }
 
-// Every lane of the wavefront: the merge of all 64 parts.
-__device__ __forceinline__ Part wave_merge(Part p, double inv_t) {
-    for (int m = 1; m < 64; m *= 2) merge(p, shuffled(p, m), inv_t);
-    return p;
-}
-
-// One workgroup per (chunk of a row, row): target rows, then draft rows.
-__global__ __launch_bounds__(kBlock) void verify_parts_kernel(VerifyArgs a, int target_rows, int chunks,
-                                                              Part* __restrict__ parts) {
-    __shared__ Part s_part[kBlock / 64];
+// One workgroup per (chunk of a row, row): target rows, then draft rows.  The
+// chunk's maximum first, then one sum against it.  A read of the logits with
+// 15 f64 operations each; 256 threads with sixteen logits each keep twice the
+// loads in flight of 512 with eight.
+constexpr int kPartBlock = 256, kPartWaves = kPartBlock / 64, kPartPer = kChunk / kPartBlock;
+template <bool GREEDY>
+__global__ __launch_bounds__(kPartBlock) void verify_parts_kernel(VerifyArgs a, int target_rows, int chunks,
+                                                                  Part* __restrict__ parts) {
+    __shared__ float s_max[kPartWaves];
+    __shared__ double s_sum[kPartWaves];
+    __shared__ int s_at[kPartWaves];
     const int r = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
     const float* row = r < target_rows ? a.target + (size_t)r * a.target_stride
                                        : a.draft + (size_t)(r - target_rows) * a.draft_stride;
-    float x[kPer];
-    float m = -INFINITY;
-    uint32_t at = 0;
-    bool ok = true;
-    const int base = chunk * kChunk + threadIdx.x;
+    const int i0 = chunk * kChunk, wave = threadIdx.x >> 6;
+    // logits 4 (t + 256 j) .. + 3 of the chunk
+    float x[kPartPer];
+    if (aligned(row) && i0 + kChunk <= a.vocab) {
 #pragma unroll
-    for (int e = 0; e < kPer; e++) {
-        const int i = base + e * kBlock;
-        x[e] = i < a.vocab ? row[i] : -INFINITY;
-        ok = ok && x[e] < INFINITY;
-        if (i < a.vocab && x[e] >= m) m = x[e], at = i;
+        for (int j = 0; j < kPartPer; j += 4) {
+            const float4 f = *(const float4*)(row + i0 + 4 * threadIdx.x + j * kPartBlock);
+            x[j] = f.x, x[j + 1] = f.y, x[j + 2] = f.z, x[j + 3] = f.w;
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < kPartPer; j++) {
+            const int i = i0 + 4 * (int)threadIdx.x + (j & ~3) * kPartBlock + (j & 3);
+            x[j] = i < a.vocab ? row[i] : -INFINITY;
+        }
     }
-    double sum = 0.0;
-    if (m != -INFINITY && a.inv_t > 0.0)
+    float m = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < kPer; e++) sum += weight(x[e], m, a.inv_t);
-    Part p = wave_merge(Part{ok ? sum : -1.0, m, at}, a.inv_t);
-    if ((threadIdx.x & 63) == 0) s_part[threadIdx.x >> 6] = p;
+    for (int j = 0; j < kPartPer; j++) m = fmaxf(m, x[j] < INFINITY ? x[j] : INFINITY);
+    m = sq_wave_max(m);
+    if ((threadIdx.x & 63) == 0) s_max[wave] = m;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kPartWaves; w++) m = fmaxf(m, s_max[w]);
+    double sum = 0.0;
+    int at = 0;
+    if constexpr (GREEDY) {
+#pragma unroll
+        for (int j = 0; j < kPartPer; j++) {
+            const int i = i0 + 4 * (int)threadIdx.x + (j & ~3) * kPartBlock + (j & 3);
+            if (i < a.vocab && x[j] == m) at = max(at, i);
+        }
+#pragma unroll
+        for (int k = 1; k < 64; k *= 2) at = max(at, __shfl_xor(at, k, 64));
+        if ((threadIdx.x & 63) == 0) s_at[wave] = at;
+    } else {
+        if (m > -INFINITY && m < INFINITY) {
+#pragma unroll
+            for (int j = 0; j < kPartPer; j++) sum += weight(x[j], m, a.inv_t);
+        }
+        sum = wave_sum64(sum);
+        if ((threadIdx.x & 63) == 0) s_sum[wave] = sum;
+    }
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int w = 1; w < kBlock / 64; w++) merge(p, s_part[w], a.inv_t);
-        parts[blockIdx.x] = p;
+#pragma unroll
+        for (int w = 1; w < kPartWaves; w++) {
+            if constexpr (GREEDY)
+                at = max(at, s_at[w]);
+            else
+                sum += s_sum[w];
+        }
+        parts[blockIdx.x] = Part{sum, m, (uint32_t)at};
     }
 }
 
@@ -122,99 +164,141 @@ struct Choice {
     uint32_t greedy;
 };
 
+// Every lane of the wavefront: a row's maximum, sum and last index of the maximum.
 __device__ __forceinline__ Part row_part(const Part* parts, size_t row, int chunks, double inv_t) {
-    Part p{0.0, -INFINITY, 0};
-    for (int c = threadIdx.x & 63; c < chunks; c += 64) merge(p, parts[row * chunks + c], inv_t);
-    return wave_merge(p, inv_t);
+    const int lane = threadIdx.x & 63;
+    float m = -INFINITY;
+    for (int c = lane; c < chunks; c += 64) m = fmaxf(m, parts[row * chunks + c].max);
+    m = sq_wave_max(m);
+    Part r{0.0, m, 0};
+    if (inv_t == 0.0) {
+        int at = 0;
+        for (int c = lane; c < chunks; c += 64)
+            if (parts[row * chunks + c].max == m) at = max(at, (int)parts[row * chunks + c].at);
+#pragma unroll
+        for (int k = 1; k < 64; k *= 2) at = max(at, __shfl_xor(at, k, 64));
+        r.at = (uint32_t)at;
+    } else if (m > -INFINITY && m < INFINITY) {
+        for (int c = lane; c < chunks; c += 64) {
+            const Part p = parts[row * chunks + c];
+            r.sum += p.sum * weight(p.max, m, inv_t);
+        }
+        r.sum = wave_sum64(r.sum);
+    }
+    return r;
 }
 
-// One wavefront: the drafts of sequence s in order, until one is rejected.
-__device__ __forceinline__ Choice choose(const VerifyBatch& b, const VerifyArgs& a, int target_rows, int s, int chunks,
-                                         const Part* parts) {
-    const int n = b.n[s];
-    const size_t t0 = b.target0[s], d0 = t0 - s;
+// One wavefront: draft i of sequence s (i = n: the row behind the last).
+// `stop`: the sequence ends here, rejected, ill or at its end.
+__device__ __forceinline__ Choice examine(const VerifyArgs& a, int target_rows, int chunks, const Part* parts, size_t t,
+                                          size_t d, bool last, int i, bool& stop) {
     Choice c{};
+    c.accepted = i;
     c.off = 0xffffffffu;
-    for (int i = 0; i <= n; i++) {
-        const Part t = row_part(parts, t0 + i, chunks, a.inv_t);
-        c.accepted = i;
-        c.t_row = (uint32_t)(t0 + i);
-        c.t_max = t.max;
-        c.t_inv = 1.0 / t.sum;
-        c.greedy = t.at;
-        if (t.sum < 0.0 || t.max == -INFINITY) {
-            c.bad = 1;
-            return c;
-        }
-        if (i == n) return c;
-        const uint32_t x = a.tokens[d0 + i];
-        if (x >= (uint32_t)a.vocab) {
-            c.bad = 2;
-            return c;
-        }
-        if (a.inv_t == 0.0) {
-            if (x != t.at) return c;
-            continue;
-        }
-        const double px = weight(a.target[(t0 + i) * a.target_stride + x], t.max, a.inv_t) * c.t_inv;
-        double qx = 1.0;
-        Part d{1.0, 0.0f, 0};
-        if (a.draft) {
-            d = row_part(parts, target_rows + d0 + i, chunks, a.inv_t);
-            if (d.sum < 0.0 || d.max == -INFINITY) {
-                c.bad = 1;
-                return c;
-            }
-            qx = weight(a.draft[(d0 + i) * a.draft_stride + x], d.max, a.inv_t) / d.sum;
-        }
-        if ((double)a.u[t0 + i] * qx < px) continue;
-        c.d_row = (uint32_t)(d0 + i);
-        c.d_max = d.max;
-        c.d_inv = a.draft ? 1.0 / d.sum : 0.0;
-        c.off = a.draft ? 0xffffffffu : x;
-        return c;
+    c.t_row = (uint32_t)t;
+    stop = true;
+    const uint32_t x = last ? 0u : a.tokens[d];
+    const bool there = x < (uint32_t)a.vocab;
+    const float lt = there ? a.target[t * a.target_stride + x] : 0.0f;
+    const bool sampled = a.draft && !last;
+    const float ld = sampled && there ? a.draft[d * a.draft_stride + x] : 0.0f;
+    const float u = last ? 0.0f : a.u[t];
+    const Part pt = row_part(parts, t, chunks, a.inv_t);
+    Part pd{1.0, 0.0f, 0};
+    if (sampled) pd = row_part(parts, target_rows + d, chunks, a.inv_t);
+    c.t_max = pt.max;
+    c.t_inv = 1.0 / pt.sum;
+    c.greedy = pt.at;
+    if (!(pt.max > -INFINITY && pt.max < INFINITY)) {
+        c.bad = 1;
+    } else if (!there) {
+        c.bad = 2;
+    } else if (last) {
+    } else if (a.inv_t == 0.0) {
+        stop = x != pt.at;
+    } else if (!(pd.max > -INFINITY && pd.max < INFINITY)) {
+        c.bad = 1;
+    } else {
+        c.d_row = (uint32_t)d;
+        c.d_max = pd.max;
+        c.d_inv = sampled ? 1.0 / pd.sum : 0.0;
+        c.off = sampled ? 0xffffffffu : x;
+        const double px = weight(lt, pt.max, a.inv_t) * c.t_inv;
+        const double qx = sampled ? weight(ld, pd.max, a.inv_t) * c.d_inv : 1.0;
+        stop = !((double)u * qx < px);
     }
     return c;
 }
 
-__device__ __forceinline__ double drawn_weight(const VerifyArgs& a, const Choice& c, int i) {
-    double w = weight(a.target[(size_t)c.t_row * a.target_stride + i], c.t_max, a.inv_t) * c.t_inv;
-    if (c.d_inv > 0.0)
-        w = fmax(w - weight(a.draft[(size_t)c.d_row * a.draft_stride + i], c.d_max, a.inv_t) * c.d_inv, 0.0);
-    return (uint32_t)i == c.off ? 0.0 : w;
+// The whole workgroup: the drafts of sequence s, one wavefront each, until one
+// ends the sequence.
+__device__ __forceinline__ Choice choose(const VerifyBatch& b, const VerifyArgs& a, int target_rows, int s, int chunks,
+                                         const Part* parts, Choice* s_c, int* s_stop) {
+    const int n = b.n[s], wave = threadIdx.x >> 6;
+    const size_t t0 = b.target0[s], d0 = t0 - s;
+    for (int i0 = 0;; i0 += kWaves) {
+        const int i = i0 + wave;
+        bool stop = false;
+        Choice c{};
+        if (i <= n) c = examine(a, target_rows, chunks, parts, t0 + i, d0 + min(i, n - 1), i == n, i, stop);
+        if ((threadIdx.x & 63) == 0) s_c[wave] = c, s_stop[wave] = stop;
+        __syncthreads();
+        // (i <= n = the last one's own stop: some round has one)
+        for (int w = 0; w < kWaves; w++)
+            if (s_stop[w]) return s_c[w];
+        __syncthreads();
+    }
 }
 
-__device__ __forceinline__ double wave_sum64(double v) {
-    for (int m = 1; m < 64; m *= 2) v += __shfl_xor(v, m, 64);
-    return v;
+// Weights of the kPer logits from i on: max(p - q, 0), or p.
+__device__ __forceinline__ void drawn_weights(const VerifyArgs& a, const Choice& c, int i, double* w) {
+#pragma clang fp contract(off)
+    float x[kPer];
+    const float* t = a.target + (size_t)c.t_row * a.target_stride;
+    load_logits(t, i, a.vocab, aligned(t), x);
+#pragma unroll
+    for (int e = 0; e < kPer; e++) w[e] = weight(x[e], c.t_max, a.inv_t) * c.t_inv;
+    if (c.d_inv > 0.0) {
+        const float* d = a.draft + (size_t)c.d_row * a.draft_stride;
+        load_logits(d, i, a.vocab, aligned(d), x);
+        // (products rounded before the difference: equal rows leave exact zeros)
+#pragma unroll
+        for (int e = 0; e < kPer; e++) {
+            const double q = weight(x[e], c.d_max, a.inv_t) * c.d_inv;
+            w[e] = fmax(w[e] - q, 0.0);
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < kPer; e++)
+        if ((uint32_t)(i + e) == c.off || i + e >= a.vocab) w[e] = 0.0;
 }
 
-// One workgroup per (chunk, sequence): the sum of the chunk's weights.
-__global__ __launch_bounds__(kBlock) void verify_sums_kernel(VerifyBatch b, VerifyArgs a, int target_rows,
+// The sums of the chunks' weights: a sequence's chunks dealt over the
+// workgroups of one grid row, each of which makes the sequence's decision for
+// itself (from parts that the L2 holds; handing it over would be a launch).
+__global__ __launch_bounds__(kBlock) void verify_sums_kernel(VerifyBatch b, VerifyArgs a, int target_rows, int chunks,
                                                              const Part* __restrict__ parts, double* __restrict__ sums,
                                                              Choice* __restrict__ choices) {
-    __shared__ Choice s_c;
-    __shared__ double s_sum[kBlock / 64];
+    __shared__ Choice s_c[kWaves];
+    __shared__ int s_stop[kWaves];
+    __shared__ double s_sum[2][kWaves];
     const int s = blockIdx.y;
-    if (threadIdx.x < 64) {
-        const Choice c = choose(b, a, target_rows, s, gridDim.x, parts);
-        if (threadIdx.x == 0) s_c = c;
-    }
-    __syncthreads();
-    const Choice c = s_c;
+    const Choice c = choose(b, a, target_rows, s, chunks, parts, s_c, s_stop);
     if (blockIdx.x == 0 && threadIdx.x == 0) choices[s] = c;
     if (c.bad || a.inv_t == 0.0) return;
-    double sum = 0.0;
-    for (int e = 0; e < kPer; e++) {
-        const int i = blockIdx.x * kChunk + e * kBlock + threadIdx.x;
-        if (i < a.vocab) sum += drawn_weight(a, c, i);
-    }
-    sum = wave_sum64(sum);
-    if ((threadIdx.x & 63) == 0) s_sum[threadIdx.x >> 6] = sum;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < kBlock / 64; w++) sum += s_sum[w];
-        sums[(size_t)s * gridDim.x + blockIdx.x] = sum;
+    int turn = 0;
+    for (int chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x, turn ^= 1) {
+        double w[kPer], sum = 0.0;
+        drawn_weights(a, c, chunk * kChunk + (int)threadIdx.x * kPer, w);
+#pragma unroll
+        for (int e = 0; e < kPer; e++) sum += w[e];
+        sum = wave_sum64(sum);
+        if ((threadIdx.x & 63) == 0) s_sum[turn][threadIdx.x >> 6] = sum;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            for (int k = 1; k < kWaves; k++) sum += s_sum[turn][k];
+            sums[(size_t)s * chunks + chunk] = sum;
+        }
     }
 }
 
@@ -224,9 +308,9 @@ __global__ __launch_bounds__(kBlock) void verify_draw_kernel(VerifyBatch b, Veri
                                                              const double* __restrict__ sums,
                                                              const Choice* __restrict__ choices,
                                                              VerifyResult* __restrict__ results) {
-    __shared__ double s_sum[kBlock], s_at, s_total;
-    __shared__ int s_chunk, s_found, s_last;
-    const int s = blockIdx.x;
+    __shared__ double s_sum[kWaves], s_at;
+    __shared__ int s_chunk, s_found[kWaves], s_last[kWaves];
+    const int s = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     Choice c = choices[s];
     VerifyResult& out = results[s];
     if (c.bad || a.inv_t == 0.0) {
@@ -234,83 +318,83 @@ __global__ __launch_bounds__(kBlock) void verify_draw_kernel(VerifyBatch b, Veri
         return;
     }
     const double u = (double)a.u[b.target0[s] + b.n[s]];
-    if (threadIdx.x == 0) {
+    const double* mine = sums + (size_t)s * chunks;
+    if (wave == 0) {
         double total = 0.0;
-        for (int i = 0; i < chunks; i++) total += sums[(size_t)s * chunks + i];
-        s_total = total;
-    }
-    __syncthreads();
-    // (p <= q everywhere, by rounding: p and q agree and the draft had neither's
-    // probability; drawn from p)
-    const bool equal = !(s_total > 0.0);
-    if (equal) c.d_inv = 0.0, c.off = 0xffffffffu;
-    auto chunk_sum = [&](int chunk) {  // of thread t: kPer consecutive logits
-        double sum = 0.0;
-        for (int e = 0; e < kPer; e++) {
-            const int i = chunk * kChunk + (int)threadIdx.x * kPer + e;
-            if (i < a.vocab) sum += drawn_weight(a, c, i);
-        }
-        return sum;
-    };
-    if (threadIdx.x == 0) {
-        double total = s_total, run = 0.0;
-        int chunk = 0, last = -1;
-        if (equal) total = 1.0;
+        for (int i = lane; i < chunks; i += 64) total += mine[i];
+        total = wave_sum64(total);
         const double at = u * total;
-        if (!equal) {
-            for (chunk = 0; chunk < chunks; chunk++) {
-                const double w = sums[(size_t)s * chunks + chunk];
-                if (w > 0.0) last = chunk;
-                if (run + w > at) break;
-                run += w;
+        double run = 0.0, before = 0.0, last_before = 0.0;
+        int chunk = -1, last = -1;
+        for (int i0 = 0; i0 < chunks && chunk < 0; i0 += 64) {
+            const double w = i0 + lane < chunks ? mine[i0 + lane] : 0.0;
+            const double upto = run + wave_scan64(w);
+            const unsigned long long over = __ballot(w > 0.0 && upto > at), some = __ballot(w > 0.0);
+            if (over) {
+                const int k = __builtin_ctzll(over);
+                chunk = i0 + k;
+                before = __shfl(upto - w, k, 64);
+            } else if (some) {
+                const int k = 63 - __builtin_clzll(some);
+                last = i0 + k;
+                last_before = __shfl(upto - w, k, 64);
             }
-            // (u near 1 and the order of the sums: the last chunk with any weight)
-            if (chunk == chunks) {
-                chunk = last;
-                run = 0.0;
-                for (int i = 0; i < chunk; i++) run += sums[(size_t)s * chunks + i];
-            }
+            run = __shfl(upto, 63, 64);
         }
-        s_chunk = chunk;
-        s_at = at - run;
-        s_found = 0x7fffffff;
-        s_last = -1;
+        // (u near 1 and the order of the sums: the last chunk with any weight)
+        if (chunk < 0) chunk = last, before = last_before;
+        if (lane == 0) {
+            s_chunk = total > 0.0 ? chunk : -1;
+            s_at = total > 0.0 ? at - before : u;
+        }
     }
     __syncthreads();
+    // (no weight anywhere: p and q agree, and neither had the draft; drawn from p, whose sum is 1)
+    const bool equal = s_chunk < 0;
+    if (equal) c.d_inv = 0.0, c.off = 0xffffffffu;
     double at = s_at;
-    for (int chunk = s_chunk; chunk < chunks; chunk++) {
-        const double mine = chunk_sum(chunk);
-        s_sum[threadIdx.x] = mine;
+    int token = 0;
+    for (int chunk = max(s_chunk, 0); chunk < chunks; chunk++) {
+        const int i = chunk * kChunk + (int)threadIdx.x * kPer;
+        double w[kPer], sum = 0.0;
+        drawn_weights(a, c, i, w);
+#pragma unroll
+        for (int e = 0; e < kPer; e++) sum += w[e];
+        // the sums before this thread's: whole wavefronts', then its own wavefront's
+        const double upto = wave_scan64(sum);
+        if (lane == 63) s_sum[wave] = upto;
         __syncthreads();
-        double before = 0.0, all = 0.0;
-        for (int t = 0; t < kBlock; t++) {
-            if (t < (int)threadIdx.x) before += s_sum[t];
-            all += s_sum[t];
+        double run = upto - sum, all = 0.0;
+        for (int k = 0; k < kWaves; k++) {
+            if (k == wave) run += all;
+            all += s_sum[k];
         }
-        double run = before;
+        int first = 0x7fffffff, last = -1;
+#pragma unroll
+        for (int e = kPer - 1; e >= 0; e--) last = last < 0 && w[e] > 0.0 ? i + e : last;
+#pragma unroll
         for (int e = 0; e < kPer; e++) {
-            const int i = chunk * kChunk + (int)threadIdx.x * kPer + e;
-            const double w = i < a.vocab ? drawn_weight(a, c, i) : 0.0;
-            run += w;
-            if (w > 0.0) {
-                atomicMax(&s_last, i);
-                if (run > at) {
-                    atomicMin(&s_found, i);
-                    break;
-                }
-            }
+            run += w[e];
+            if (w[e] > 0.0 && run > at) first = min(first, i + e);
         }
+#pragma unroll
+        for (int k = 1; k < 64; k *= 2) {
+            first = min(first, __shfl_xor(first, k, 64));
+            last = max(last, __shfl_xor(last, k, 64));
+        }
+        if (lane == 0) s_found[wave] = first, s_last[wave] = last;
         __syncthreads();
-        const bool done = s_found != 0x7fffffff || (!equal && s_last >= 0);
-        if (done) break;
+        for (int k = 0; k < kWaves; k++) first = min(first, s_found[k]), last = max(last, s_last[k]);
+        if (last >= 0) token = last;
+        if (first != 0x7fffffff) token = first;
+        if (first != 0x7fffffff || (!equal && last >= 0)) break;
         at -= all;
         __syncthreads();
     }
-    if (threadIdx.x == 0) {
-        const int t = s_found != 0x7fffffff ? s_found : s_last;
-        out = VerifyResult{c.accepted, (uint32_t)(t < 0 ? c.greedy : t), 0, 0};
-    }
+    if (threadIdx.x == 0) out = VerifyResult{c.accepted, (uint32_t)token, 0, 0};
 }
+
+constexpr int kSumGroups = 512;  // workgroups of the sums' launch, about two a CU
 
 size_t align16(size_t n) { return (n + 15) & ~(size_t)15; }
 
@@ -328,10 +412,11 @@ int launch_verify(hipStream_t s, const VerifyBatch& b, const VerifyArgs& a, size
     Part* parts = (Part*)ws;
     double* sums = (double*)((char*)ws + align16(rows * chunks * sizeof(Part)));
     Choice* choices = (Choice*)((char*)sums + align16((size_t)b.n_seqs * chunks * sizeof(double)));
-    hipLaunchKernelGGL(verify_parts_kernel, dim3((unsigned)(rows * chunks)), dim3(kBlock), 0, s, a, (int)target_rows,
-                       chunks, parts);
-    hipLaunchKernelGGL(verify_sums_kernel, dim3(chunks, b.n_seqs), dim3(kBlock), 0, s, b, a, (int)target_rows,
-                       (const Part*)parts, sums, choices);
+    if (rows * chunks > (size_t)INT32_MAX) return set_error(SQ_ERR_SHAPE, "verify_draft: ShapeMismatch (too many logits)");
+    auto kernel = a.inv_t == 0.0 ? verify_parts_kernel<true> : verify_parts_kernel<false>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(rows * chunks)), dim3(kPartBlock), 0, s, a, (int)target_rows, chunks, parts);
+    hipLaunchKernelGGL(verify_sums_kernel, dim3(std::min(chunks, std::max(1, kSumGroups / (int)b.n_seqs)), b.n_seqs),
+                       dim3(kBlock), 0, s, b, a, (int)target_rows, chunks, (const Part*)parts, sums, choices);
     hipLaunchKernelGGL(verify_draw_kernel, dim3(b.n_seqs), dim3(kBlock), 0, s, b, a, chunks, (const double*)sums,
                        (const Choice*)choices, results);
     return check_launch("verify");

@@ -119,4 +119,53 @@ void scratch_trim() {
     for (const Block& b : drop) (void)hipFree(b.p);
 }
 
+namespace {
+
+constexpr size_t kPinnedKeep = 16;       // idle blocks kept per device
+constexpr size_t kPinnedMost = 1 << 20;  // larger ones are never kept
+Pool& pinned_of(int device) {
+    static Pool* pools = new Pool[kMaxDevices];
+    return pools[device];
+}
+
+}  // namespace
+
+int PinnedTmp::alloc(size_t n) {
+    SQ_HIP_CHECK(hipGetDevice(&device));
+    if (device >= 0 && device < kMaxDevices) {
+        Pool& P = pinned_of(device);
+        std::lock_guard<std::mutex> lk(P.mu);
+        for (size_t i = 0; i < P.idle.size(); i++)
+            if (P.idle[i].size >= n) {
+                p = P.idle[i].p;
+                size = P.idle[i].size;
+                P.idle[i] = P.idle.back();
+                P.idle.pop_back();
+                return 0;
+            }
+    }
+    const size_t want = rounded(n ? n : 1);
+    const hipError_t e = hipHostMalloc(&p, want, hipHostMallocDefault);
+    if (e != hipSuccess) {
+        (void)hipGetLastError();
+        p = nullptr;
+        return set_error(SQ_ERR_HIP, std::string("hipHostMalloc: ") + hipGetErrorString(e));
+    }
+    size = want;
+    return 0;
+}
+
+PinnedTmp::~PinnedTmp() {
+    if (!p) return;
+    if (device >= 0 && device < kMaxDevices && size <= kPinnedMost) {
+        Pool& P = pinned_of(device);
+        std::lock_guard<std::mutex> lk(P.mu);
+        if (P.idle.size() < kPinnedKeep) {
+            P.idle.push_back(Block{p, size, 0});
+            return;
+        }
+    }
+    (void)hipHostFree(p);
+}
+
 }  // namespace sq

@@ -39,4 +39,18 @@ struct Tmp {
     int alloc(size_t n) { return scratch_get(n, &p, &size, &device); }
 };
 
+// Pinned host memory for what a call's kernels report to the host (a copy back
+// costs 8 to 10 us of a call): kept between calls like the device blocks.
+// Written by kernels, read by the host once they have ended.
+struct PinnedTmp {
+    void* p = nullptr;
+    size_t size = 0;
+    int device = 0;
+    PinnedTmp() = default;
+    PinnedTmp(const PinnedTmp&) = delete;
+    PinnedTmp& operator=(const PinnedTmp&) = delete;
+    ~PinnedTmp();
+    int alloc(size_t n);
+};
+
 }  // namespace sq

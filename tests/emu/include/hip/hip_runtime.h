@@ -201,6 +201,23 @@ inline int any(bool p) {
     return 0;
 }
 
+inline unsigned long long ballot(bool p) {
+    const uint64_t* all = wave_exchange(p ? 1 : 0, 0x5001);
+    unsigned long long r = 0;
+    for (int l = 0; l < 64; l++) r |= (unsigned long long)(all[l] & 1) << l;
+    return r;
+}
+template <typename T>
+inline T shfl_up(T v, int by) {
+    const uint64_t* all = wave_exchange(to_bits(v), 0x5100 + by);
+    return from_bits<T>(all[g_lane >= by ? g_lane - by : g_lane]);
+}
+template <typename T>
+inline T shfl(T v, int from) {
+    const uint64_t* all = wave_exchange(to_bits(v), 0x5002);
+    return from_bits<T>(all[from & 63]);
+}
+
 // v_perm_b32: byte i of the result is byte sel_i of {s1 (0-3), s0 (4-7)}.
 inline unsigned perm(unsigned s0, unsigned s1, unsigned sel) {
     unsigned r = 0;
@@ -385,6 +402,9 @@ inline sqemu_v16f mfma_f32_32x32x8f16(sqemu_v4h a, sqemu_v4h b, sqemu_v16f c) {
 // v_exp_f32 (2^x): the host exp2f stands in for the device instruction
 #define __builtin_amdgcn_exp2f(x) ::exp2f((float)(x))
 #define __builtin_amdgcn_logf(x) ::log2f((float)(x))
+#define __ballot(p) ::sqemu::ballot((p) != 0)
+#define __shfl_up(v, by, w) ::sqemu::shfl_up((v), (by))
+#define __shfl(v, from, w) ::sqemu::shfl((v), (from))
 #define __any(p) ::sqemu::any((p) != 0)
 #define __builtin_amdgcn_perm(a, b, s) ::sqemu::perm((a), (b), (s))
 #define __builtin_amdgcn_sdot4(a, b, c, cl) ::sqemu::sdot4((a), (b), (c), (cl))
