@@ -39,105 +39,148 @@ __device__ __forceinline__ double wave_max64(double v) {
     return v;
 }
 
-// rint(x / scale) as the stored byte
-__device__ __forceinline__ uint32_t quant(double x, double scale) {
-    double q = scale > 0.0 ? rint(x / scale) : 0.0;
-    q = fmin(fmax(q, -127.0), 127.0);
-    return (uint32_t)((int)q + 128);
+// x / s rounded as a division is, from r = 1 / s: the product is off by its last
+// bits, and the remainder, which is exact, corrects it (a quotient that is a
+// whole and a half comes out as that, so ties go where a division's go).
+__device__ __forceinline__ double divide(double x, double s, double r) {
+    const double y = x * r;
+    return fma(fma(-y, s, x), r, y);
+}
+// rint(x / s) as the stored byte; r = 0: a scale of 0, whose values are zeros
+__device__ __forceinline__ uint32_t quant(double x, double s, double r) {
+    return (uint32_t)((int)fmin(fmax(rint(divide(x, s, r)), -127.0), 127.0) + 128);
 }
 // a stored byte in the steps of a larger scale
-__device__ __forceinline__ uint32_t requant(uint32_t b, double from, double to) {
-    return (uint32_t)((int)rint((double)((int)b - 128) * from / to) + 128);
+__device__ __forceinline__ uint32_t requant(uint32_t b, double from, double s, double r) {
+    return (uint32_t)((int)rint(divide((double)((int)b - 128) * from, s, r)) + 128);
 }
+__device__ __forceinline__ double reciprocal(double s) { return s > 0.0 ? 1.0 / s : 0.0; }
 
-// One workgroup per (written page, KV head).  Thread t has position t / 4 of
-// the page and dimensions 16 (t % 4) .. + 15 of each 64: one 16-byte piece of
-// the keys' order.
+constexpr int kFewTokens = 16;
+
+// One workgroup per (written page, KV head).  A wavefront's lanes have pairs of
+// dimensions, HD / 2 threads a position and eight positions at a time, so a
+// single decoded token is one load of each.  The page's maxima first (the
+// values stay in registers), then:
+//   few new rows and no scale that grows: their bytes go where they belong, one
+//   by one (a wavefront's keys are 2 bytes a lane, its values 1);
+//   otherwise through an image of the page in LDS, written out 16 bytes a
+//   thread; earlier rows of the page are in it, in the steps of the new scale.
+// Bound by latency for single tokens, by the f64 operations (about 20 a value)
+// and the reads for whole pages.
 template <int HD>
-__global__ __launch_bounds__(kBlock) void kv_append_kernel(KvView kv, const KvItem* __restrict__ items,
+__global__ __launch_bounds__(HD * 4) void kv_append_kernel(KvView kv, const KvItem* __restrict__ items,
                                                            const double2* __restrict__ rope, int half,
                                                            const float* __restrict__ k, size_t k_stride,
                                                            const float* __restrict__ v, size_t v_stride,
                                                            uint32_t* bad) {
-    constexpr int C = HD / 64;
-    __shared__ double s_max[2][kBlock / 64];
-    const KvItem it = items[blockIdx.x / kv.kv_heads];
-    const int head = blockIdx.x % kv.kv_heads;
+    constexpr int NT = HD * 4, PAIRS = HD / 2, PASSES = kPage / 8, BYTES = kPage * HD;
+    __shared__ double s_max[2][NT / 64];
+    __shared__ __attribute__((aligned(16))) uint8_t s_img[2][BYTES];
+    const int at = blockIdx.x / kv.kv_heads, head = blockIdx.x - at * kv.kv_heads;
+    const KvItem it = items[at];
     const size_t cell = (size_t)it.page * kv.kv_heads + head;
-    uint8_t* kb = kv.bytes + cell * 2 * kPage * HD;
-    uint8_t* vb = kb + kPage * HD;
-    const int tok = threadIdx.x >> 2, g = threadIdx.x & 3;
-    const int i = tok - it.tok0;
-    const bool mine = i >= 0 && i < it.n;
-    double x[C][16], y[C][16];
+    uint8_t* page = kv.bytes + cell * 2 * BYTES;  // keys, then values
+    const float2 old = it.tok0 ? kv.scales[cell] : make_float2(0.0f, 0.0f);
+    const int d = 2 * (threadIdx.x % PAIRS), first = threadIdx.x / PAIRS;
+    const bool vec = (((uintptr_t)k | (uintptr_t)v | (k_stride * 4) | (v_stride * 4)) & 7) == 0;
+    double x[PASSES][2], y[PASSES][2];
     double kmax = 0.0, vmax = 0.0;
     bool ok = true;
 #pragma unroll
-    for (int c = 0; c < C; c++)
-#pragma unroll
-        for (int e = 0; e < 16; e += 2) {
-            const int d = 64 * c + 16 * g + e;
-            double a = 0.0, b = 0.0, p = 0.0, q = 0.0;
-            if (mine) {
-                const size_t row = it.row0 + i;
-                const float* kr = k + row * k_stride + (size_t)head * HD + d;
-                const float* vr = v + row * v_stride + (size_t)head * HD + d;
-                a = kr[0], b = kr[1], p = vr[0], q = vr[1];
-                // values that are not finite are reported and stored as zero: in
-                // the page's scale they would take the other positions with them
-                if (!(fabs(a) < INFINITY && fabs(b) < INFINITY)) a = b = 0.0, ok = false;
-                if (!(fabs(p) < INFINITY)) p = 0.0, ok = false;
-                if (!(fabs(q) < INFINITY)) q = 0.0, ok = false;
-                if (rope && d / 2 < half) {
-                    const double2 cs = rope[row * half + d / 2];
-                    const double t = a * cs.x - b * cs.y;
-                    b = a * cs.y + b * cs.x;
-                    a = t;
-                }
+    for (int p = 0; p < PASSES; p++) {
+        const int i = first + 8 * p;  // the new row
+        float a = 0.0f, b = 0.0f, e = 0.0f, f = 0.0f;
+        double2 cs{1.0, 0.0};
+        if (i < it.n) {
+            const size_t row = (size_t)it.row0 + i;
+            const float* kr = k + row * k_stride + (size_t)head * HD + d;
+            const float* vr = v + row * v_stride + (size_t)head * HD + d;
+            if (vec) {
+                const float2 t = *(const float2*)kr, w = *(const float2*)vr;
+                a = t.x, b = t.y, e = w.x, f = w.y;
+            } else {
+                a = kr[0], b = kr[1], e = vr[0], f = vr[1];
             }
-            x[c][e] = a, x[c][e + 1] = b, y[c][e] = p, y[c][e + 1] = q;
-            kmax = fmax(kmax, fmax(fabs(a), fabs(b)));
-            vmax = fmax(vmax, fmax(fabs(p), fabs(q)));
+            if (rope && d / 2 < half) cs = rope[row * half + d / 2];
         }
+        // values that are not finite are reported and stored as zero: in the
+        // page's scale they would take the other positions with them
+        if (!(fabsf(a) < INFINITY && fabsf(b) < INFINITY)) a = b = 0.0f, ok = false;
+        if (!(fabsf(e) < INFINITY)) e = 0.0f, ok = false;
+        if (!(fabsf(f) < INFINITY)) f = 0.0f, ok = false;
+        x[p][0] = (double)a * cs.x - (double)b * cs.y;
+        x[p][1] = (double)a * cs.y + (double)b * cs.x;
+        y[p][0] = e, y[p][1] = f;
+        kmax = fmax(kmax, fmax(fabs(x[p][0]), fabs(x[p][1])));
+        vmax = fmax(vmax, fmax(fabs(y[p][0]), fabs(y[p][1])));
+    }
     if (!ok) *bad = 1u;
     kmax = wave_max64(kmax);
     vmax = wave_max64(vmax);
     if ((threadIdx.x & 63) == 0) s_max[0][threadIdx.x >> 6] = kmax, s_max[1][threadIdx.x >> 6] = vmax;
-    const float2 old = it.tok0 ? kv.scales[cell] : make_float2(0.0f, 0.0f);
     __syncthreads();
-    for (int w = 0; w < kBlock / 64; w++) kmax = fmax(kmax, s_max[0][w]), vmax = fmax(vmax, s_max[1][w]);
+#pragma unroll
+    for (int w = 0; w < NT / 64; w++) kmax = fmax(kmax, s_max[0][w]), vmax = fmax(vmax, s_max[1][w]);
     const float ks = fmaxf(old.x, (float)(kmax / 127.0)), vs = fmaxf(old.y, (float)(vmax / 127.0));
-    if (it.tok0 && (ks > old.x || vs > old.y)) {
-        // earlier rows of the page, in the steps of the larger scales
-        for (int e = threadIdx.x; e < it.tok0 * HD; e += kBlock) {
-            const int t = e / HD, d = e % HD;
-            uint8_t* pk = kb + kv_k_off(t, d, HD);
-            uint8_t* pv = vb + kv_v_off(t, d);
-            if (ks > old.x) *pk = (uint8_t)requant(*pk, old.x, ks);
-            if (vs > old.y) *pv = (uint8_t)requant(*pv, old.y, vs);
-        }
-    }
+    const double kr = reciprocal(ks), vr = reciprocal(vs);
+    const bool grown = it.tok0 && (ks > old.x || vs > old.y);
     if (threadIdx.x == 0) kv.scales[cell] = make_float2(ks, vs);
-    if (!mine) return;
+    if (it.n <= kFewTokens && !grown) {
 #pragma unroll
-    for (int c = 0; c < C; c++)
-#pragma unroll
-        for (int e = 0; e < 16; e++) {
-            const int d = 64 * c + 16 * g + e;
-            kb[kv_k_off(tok, d, HD)] = (uint8_t)quant(x[c][e], ks);
-            vb[kv_v_off(tok, d)] = (uint8_t)quant(y[c][e], vs);
+        for (int p = 0; p < kFewTokens / 8; p++) {
+            const int i = first + 8 * p, tok = it.tok0 + i;
+            if (i >= it.n) continue;
+            *(uint16_t*)(page + kv_k_off(tok, d, HD)) = (uint16_t)(quant(x[p][0], ks, kr) | quant(x[p][1], ks, kr) << 8);
+            page[BYTES + kv_v_off(tok, d)] = (uint8_t)quant(y[p][0], vs, vr);
+            page[BYTES + kv_v_off(tok, d + 1)] = (uint8_t)quant(y[p][1], vs, vr);
         }
+        return;
+    }
+    // the image's 16-byte pieces: the page's as they are where it has earlier rows
+    constexpr int PIECES = BYTES / 16;
+    if (it.tok0) {
+        for (int e = threadIdx.x; e < 2 * PIECES; e += NT) ((uint4*)s_img)[e] = ((const uint4*)page)[e];
+        __syncthreads();
+        if (grown)
+            for (int e = threadIdx.x; e < it.tok0 * HD; e += NT) {
+                const int t = e / HD, c = e % HD;
+                uint8_t* pk = &s_img[0][kv_k_off(t, c, HD)];
+                uint8_t* pv = &s_img[1][kv_v_off(t, c)];
+                if (ks > old.x) *pk = (uint8_t)requant(*pk, old.x, ks, kr);
+                if (vs > old.y) *pv = (uint8_t)requant(*pv, old.y, vs, vr);
+            }
+    }
+#pragma unroll
+    for (int p = 0; p < PASSES; p++) {
+        const int i = first + 8 * p, tok = it.tok0 + i;
+        if (i >= it.n) continue;
+        *(uint16_t*)&s_img[0][kv_k_off(tok, d, HD)] = (uint16_t)(quant(x[p][0], ks, kr) | quant(x[p][1], ks, kr) << 8);
+        s_img[1][kv_v_off(tok, d)] = (uint8_t)quant(y[p][0], vs, vr);
+        s_img[1][kv_v_off(tok, d + 1)] = (uint8_t)quant(y[p][1], vs, vr);
+    }
+    __syncthreads();
+    // (positions behind the new rows are nobody's: what the image holds there goes along)
+    for (int e = threadIdx.x; e < 2 * PIECES; e += NT) ((uint4*)page)[e] = ((const uint4*)s_img)[e];
 }
 
-// One workgroup per (sequence, page of its last positions, KV head).
+// One workgroup per (sequence, page of its last positions, KV head): the page's
+// bytes through LDS, four dimensions a thread on the way out.
+template <int HD>
 __global__ __launch_bounds__(kBlock) void kv_read_kernel(KvView kv, KvPlanView p, int last, float* __restrict__ k_out,
                                                          float* __restrict__ v_out) {
+    constexpr int BYTES = kPage * HD, PIECES = BYTES / 16, Q = HD / 4;
+    __shared__ __attribute__((aligned(16))) uint8_t s_img[2][BYTES];
     __shared__ int s_row;
-    const int head = blockIdx.x % kv.kv_heads, j = blockIdx.x / kv.kv_heads, seq = blockIdx.y;
+    const int j = blockIdx.x / kv.kv_heads, head = blockIdx.x - j * kv.kv_heads, seq = blockIdx.y;
     const KvSeq s = p.seqs[seq];
     const int len = s.past + s.n_new, first = len > last ? len - last : 0;
     const int page = first / kPage + j;
     if (page * kPage >= len) return;
+    const size_t cell = (size_t)p.pages[s.table0 + page] * kv.kv_heads + head;
+    const float2 scale = kv.scales[cell];
+    const uint4* from = (const uint4*)(kv.bytes + cell * 2 * BYTES);
+    for (int e = threadIdx.x; e < 2 * PIECES; e += kBlock) ((uint4*)s_img)[e] = from[e];
     if (threadIdx.x == 0) s_row = 0;
     __syncthreads();
     // rows of the sequences before this one
@@ -148,17 +191,28 @@ __global__ __launch_bounds__(kBlock) void kv_read_kernel(KvView kv, KvPlanView p
     }
     if (before) atomicAdd(&s_row, before);
     __syncthreads();
-    const size_t row0 = (size_t)s_row, width = (size_t)kv.kv_heads * kv.head_dim;
-    const size_t cell = (size_t)p.pages[s.table0 + page] * kv.kv_heads + head;
-    const float2 scale = kv.scales[cell];
-    const uint8_t* kb = kv.bytes + cell * 2 * kPage * kv.head_dim;
-    const uint8_t* vb = kb + kPage * kv.head_dim;
-    for (int e = threadIdx.x; e < kPage * kv.head_dim; e += kBlock) {
-        const int tok = e / kv.head_dim, d = e % kv.head_dim, pos = page * kPage + tok;
-        if (pos < first || pos >= len) continue;
-        const size_t o = (row0 + pos - first) * width + (size_t)head * kv.head_dim + d;
-        if (k_out) k_out[o] = (float)((int)kb[kv_k_off(tok, d, kv.head_dim)] - 128) * scale.x;
-        if (v_out) v_out[o] = (float)((int)vb[kv_v_off(tok, d)] - 128) * scale.y;
+    const size_t row0 = (size_t)s_row, width = (size_t)kv.kv_heads * HD;
+    const int lo = max(first - page * kPage, 0), hi = min(len - page * kPage, kPage);
+    for (int e = lo * Q + threadIdx.x; e < hi * Q; e += kBlock) {
+        const int tok = e / Q, d = e % Q * 4;
+        const size_t o = (row0 + page * kPage + tok - first) * width + (size_t)head * HD + d;
+        const uint32_t kw = *(const uint32_t*)&s_img[0][kv_k_off(tok, d, HD)];
+        float a[4], b[4];
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+            a[c] = (float)((int)((kw >> (8 * c)) & 255u) - 128) * scale.x;
+            b[c] = (float)((int)s_img[1][kv_v_off(tok, d + c)] - 128) * scale.y;
+        }
+        auto store = [](float* out, const float* w) {
+            if (((uintptr_t)out & 15) == 0) {
+                *(float4*)out = make_float4(w[0], w[1], w[2], w[3]);
+            } else {
+#pragma unroll
+                for (int c = 0; c < 4; c++) out[c] = w[c];
+            }
+        };
+        if (k_out) store(k_out + o, a);
+        if (v_out) store(v_out + o, b);
     }
 }
 
@@ -175,11 +229,11 @@ int launch_kv_append(hipStream_t s, const KvView& kv, const KvPlanView& p, const
     const size_t grid = (size_t)p.n_items * kv.kv_heads;
     if (grid > (size_t)INT32_MAX) return set_error(SQ_ERR_SHAPE, "kv_append: ShapeMismatch (too many pages)");
     if (kv.head_dim == 64)
-        hipLaunchKernelGGL(kv_append_kernel<64>, dim3((unsigned)grid), dim3(kBlock), 0, s, kv, p.items,
-                           p.rope, p.half, k, k_stride, v, v_stride, bad);
+        hipLaunchKernelGGL(kv_append_kernel<64>, dim3((unsigned)grid), dim3(256), 0, s, kv, p.items, p.rope,
+                           p.half, k, k_stride, v, v_stride, bad);
     else
-        hipLaunchKernelGGL(kv_append_kernel<128>, dim3((unsigned)grid), dim3(kBlock), 0, s, kv, p.items,
-                           p.rope, p.half, k, k_stride, v, v_stride, bad);
+        hipLaunchKernelGGL(kv_append_kernel<128>, dim3((unsigned)grid), dim3(512), 0, s, kv, p.items, p.rope,
+                           p.half, k, k_stride, v, v_stride, bad);
     return check_launch("kv_append");
 }
 
@@ -187,7 +241,10 @@ int launch_kv_read(hipStream_t s, const KvView& kv, const KvPlanView& p, int las
                    float* v_out) {
     const size_t grid = (size_t)max_pages * kv.kv_heads;
     if (grid > (size_t)INT32_MAX) return set_error(SQ_ERR_SHAPE, "kv_read: ShapeMismatch (too many pages)");
-    hipLaunchKernelGGL(kv_read_kernel, dim3((unsigned)grid, p.n_seqs), dim3(kBlock), 0, s, kv, p, last, k_out, v_out);
+    if (kv.head_dim == 64)
+        hipLaunchKernelGGL(kv_read_kernel<64>, dim3((unsigned)grid, p.n_seqs), dim3(kBlock), 0, s, kv, p, last, k_out, v_out);
+    else
+        hipLaunchKernelGGL(kv_read_kernel<128>, dim3((unsigned)grid, p.n_seqs), dim3(kBlock), 0, s, kv, p, last, k_out, v_out);
     return check_launch("kv_read");
 }
 
