@@ -14,8 +14,6 @@
 namespace sq {
 namespace {
 
-constexpr int kBlock = 256;
-
 inline int check_launch(const char* what) {
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return set_error(SQ_ERR_HIP, std::string(what) + ": " + hipGetErrorString(e));
@@ -58,161 +56,165 @@ __device__ __forceinline__ double reciprocal(double s) { return s > 0.0 ? 1.0 / 
 
 constexpr int kFewTokens = 16;
 
-// One workgroup per (written page, KV head).  A wavefront's lanes have pairs of
-// dimensions, HD / 2 threads a position and eight positions at a time, so a
-// single decoded token is one load of each.  The page's maxima first (the
-// values stay in registers), then:
-//   few new rows and no scale that grows: their bytes go where they belong, one
-//   by one (a wavefront's keys are 2 bytes a lane, its values 1);
+// One workgroup per (written page, KV head) and one of keys and values.  A
+// wavefront's lanes have pairs of dimensions, HD / 2 threads a position and
+// eight positions at a time, so a single decoded token is one load of each.
+// The page's maximum first (the values stay in registers), then:
+//   few new rows and no scale that grows: their bytes go where they belong (2
+//   bytes of keys a lane, or two single ones of values);
 //   otherwise through an image of the page in LDS, written out 16 bytes a
 //   thread; earlier rows of the page are in it, in the steps of the new scale.
-// Bound by latency for single tokens, by the f64 operations (about 20 a value)
-// and the reads for whole pages.
+// Bound by latency for single tokens, by the reads and about 20 f64 operations
+// a value for whole pages.  (Keys and values in one workgroup: 10.7 us for 2011
+// rows of 8 x 128, one page of a head a CU with nothing to overlap.)
+template <int HD, bool VALUES>
+__device__ __forceinline__ void append_page(const KvView& kv, const KvItem& it, int head,
+                                            const double2* __restrict__ rope, int half, const float* __restrict__ in,
+                                            size_t stride, uint32_t* bad, double* s_max, uint8_t* s_img) {
+    constexpr int NT = HD * 4, PAIRS = HD / 2, PASSES = kPage / 8, BYTES = kPage * HD;
+    const size_t cell = (size_t)it.page * kv.kv_heads + head;
+    uint8_t* page = kv.bytes + (cell * 2 + VALUES) * BYTES;
+    float* scale = (float*)(kv.scales + cell) + VALUES;
+    const float old = it.tok0 ? *scale : 0.0f;
+    const int d = 2 * (threadIdx.x % PAIRS), first = threadIdx.x / PAIRS;
+    const bool vec = (((uintptr_t)in | (stride * 4)) & 7) == 0;
+    double x[PASSES][2];
+    double top = 0.0;
+    bool ok = true;
+#pragma unroll
+    for (int p = 0; p < PASSES; p++) {
+        const int i = first + 8 * p;  // the new row
+        float a = 0.0f, b = 0.0f;
+        double2 cs{1.0, 0.0};
+        if (i < it.n) {
+            const size_t row = (size_t)it.row0 + i;
+            const float* r = in + row * stride + (size_t)head * HD + d;
+            if (vec) {
+                const float2 t = *(const float2*)r;
+                a = t.x, b = t.y;
+            } else {
+                a = r[0], b = r[1];
+            }
+            if (!VALUES && rope && d / 2 < half) cs = rope[row * half + d / 2];
+        }
+        // values that are not finite are reported and stored as zero: in the
+        // page's scale they would take the other positions with them
+        if (!(fabsf(a) < INFINITY)) a = 0.0f, b = VALUES ? b : 0.0f, ok = false;
+        if (!(fabsf(b) < INFINITY)) b = 0.0f, a = VALUES ? a : 0.0f, ok = false;
+        if constexpr (VALUES) {
+            x[p][0] = a, x[p][1] = b;
+        } else {
+            x[p][0] = (double)a * cs.x - (double)b * cs.y;
+            x[p][1] = (double)a * cs.y + (double)b * cs.x;
+        }
+        top = fmax(top, fmax(fabs(x[p][0]), fabs(x[p][1])));
+    }
+    if (!ok) *bad = 1u;
+    top = wave_max64(top);
+    if ((threadIdx.x & 63) == 0) s_max[threadIdx.x >> 6] = top;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < NT / 64; w++) top = fmax(top, s_max[w]);
+    const float s = fmaxf(old, (float)(top / 127.0));
+    const double r = reciprocal(s);
+    const bool grown = it.tok0 && s > old;
+    if (threadIdx.x == 0) *scale = s;
+    auto put = [&](uint8_t* to, int tok, const double* v) {
+        const uint32_t b0 = quant(v[0], s, r), b1 = quant(v[1], s, r);
+        if constexpr (VALUES) {
+            to[kv_v_off(tok, d)] = (uint8_t)b0;
+            to[kv_v_off(tok, d + 1)] = (uint8_t)b1;
+        } else {
+            *(uint16_t*)&to[kv_k_off(tok, d, HD)] = (uint16_t)(b0 | b1 << 8);
+        }
+    };
+    if (it.n <= kFewTokens && !grown) {
+#pragma unroll
+        for (int p = 0; p < kFewTokens / 8; p++)
+            if (first + 8 * p < it.n) put(page, it.tok0 + first + 8 * p, x[p]);
+        return;
+    }
+    // the image's 16-byte pieces: the page's as they are where it has earlier rows
+    constexpr int PIECES = BYTES / 16;
+    if (it.tok0) {
+        for (int e = threadIdx.x; e < PIECES; e += NT) ((uint4*)s_img)[e] = ((const uint4*)page)[e];
+        __syncthreads();
+        if (grown)
+            for (int e = threadIdx.x; e < it.tok0 * HD; e += NT) {
+                uint8_t* b = &s_img[VALUES ? kv_v_off(e / HD, e % HD) : kv_k_off(e / HD, e % HD, HD)];
+                *b = (uint8_t)requant(*b, old, s, r);
+            }
+    }
+#pragma unroll
+    for (int p = 0; p < PASSES; p++)
+        if (first + 8 * p < it.n) put(s_img, it.tok0 + first + 8 * p, x[p]);
+    __syncthreads();
+    // (positions behind the new rows are nobody's: what the image holds there goes along)
+    for (int e = threadIdx.x; e < PIECES; e += NT) ((uint4*)page)[e] = ((const uint4*)s_img)[e];
+}
+
 template <int HD>
 __global__ __launch_bounds__(HD * 4) void kv_append_kernel(KvView kv, const KvItem* __restrict__ items,
                                                            const double2* __restrict__ rope, int half,
                                                            const float* __restrict__ k, size_t k_stride,
                                                            const float* __restrict__ v, size_t v_stride,
                                                            uint32_t* bad) {
-    constexpr int NT = HD * 4, PAIRS = HD / 2, PASSES = kPage / 8, BYTES = kPage * HD;
-    __shared__ double s_max[2][NT / 64];
-    __shared__ __attribute__((aligned(16))) uint8_t s_img[2][BYTES];
+    __shared__ double s_max[HD * 4 / 64];
+    __shared__ __attribute__((aligned(16))) uint8_t s_img[kPage * HD];
     const int at = blockIdx.x / kv.kv_heads, head = blockIdx.x - at * kv.kv_heads;
     const KvItem it = items[at];
-    const size_t cell = (size_t)it.page * kv.kv_heads + head;
-    uint8_t* page = kv.bytes + cell * 2 * BYTES;  // keys, then values
-    const float2 old = it.tok0 ? kv.scales[cell] : make_float2(0.0f, 0.0f);
-    const int d = 2 * (threadIdx.x % PAIRS), first = threadIdx.x / PAIRS;
-    const bool vec = (((uintptr_t)k | (uintptr_t)v | (k_stride * 4) | (v_stride * 4)) & 7) == 0;
-    double x[PASSES][2], y[PASSES][2];
-    double kmax = 0.0, vmax = 0.0;
-    bool ok = true;
-#pragma unroll
-    for (int p = 0; p < PASSES; p++) {
-        const int i = first + 8 * p;  // the new row
-        float a = 0.0f, b = 0.0f, e = 0.0f, f = 0.0f;
-        double2 cs{1.0, 0.0};
-        if (i < it.n) {
-            const size_t row = (size_t)it.row0 + i;
-            const float* kr = k + row * k_stride + (size_t)head * HD + d;
-            const float* vr = v + row * v_stride + (size_t)head * HD + d;
-            if (vec) {
-                const float2 t = *(const float2*)kr, w = *(const float2*)vr;
-                a = t.x, b = t.y, e = w.x, f = w.y;
-            } else {
-                a = kr[0], b = kr[1], e = vr[0], f = vr[1];
-            }
-            if (rope && d / 2 < half) cs = rope[row * half + d / 2];
-        }
-        // values that are not finite are reported and stored as zero: in the
-        // page's scale they would take the other positions with them
-        if (!(fabsf(a) < INFINITY && fabsf(b) < INFINITY)) a = b = 0.0f, ok = false;
-        if (!(fabsf(e) < INFINITY)) e = 0.0f, ok = false;
-        if (!(fabsf(f) < INFINITY)) f = 0.0f, ok = false;
-        x[p][0] = (double)a * cs.x - (double)b * cs.y;
-        x[p][1] = (double)a * cs.y + (double)b * cs.x;
-        y[p][0] = e, y[p][1] = f;
-        kmax = fmax(kmax, fmax(fabs(x[p][0]), fabs(x[p][1])));
-        vmax = fmax(vmax, fmax(fabs(y[p][0]), fabs(y[p][1])));
-    }
-    if (!ok) *bad = 1u;
-    kmax = wave_max64(kmax);
-    vmax = wave_max64(vmax);
-    if ((threadIdx.x & 63) == 0) s_max[0][threadIdx.x >> 6] = kmax, s_max[1][threadIdx.x >> 6] = vmax;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < NT / 64; w++) kmax = fmax(kmax, s_max[0][w]), vmax = fmax(vmax, s_max[1][w]);
-    const float ks = fmaxf(old.x, (float)(kmax / 127.0)), vs = fmaxf(old.y, (float)(vmax / 127.0));
-    const double kr = reciprocal(ks), vr = reciprocal(vs);
-    const bool grown = it.tok0 && (ks > old.x || vs > old.y);
-    if (threadIdx.x == 0) kv.scales[cell] = make_float2(ks, vs);
-    if (it.n <= kFewTokens && !grown) {
-#pragma unroll
-        for (int p = 0; p < kFewTokens / 8; p++) {
-            const int i = first + 8 * p, tok = it.tok0 + i;
-            if (i >= it.n) continue;
-            *(uint16_t*)(page + kv_k_off(tok, d, HD)) = (uint16_t)(quant(x[p][0], ks, kr) | quant(x[p][1], ks, kr) << 8);
-            page[BYTES + kv_v_off(tok, d)] = (uint8_t)quant(y[p][0], vs, vr);
-            page[BYTES + kv_v_off(tok, d + 1)] = (uint8_t)quant(y[p][1], vs, vr);
-        }
-        return;
-    }
-    // the image's 16-byte pieces: the page's as they are where it has earlier rows
-    constexpr int PIECES = BYTES / 16;
-    if (it.tok0) {
-        for (int e = threadIdx.x; e < 2 * PIECES; e += NT) ((uint4*)s_img)[e] = ((const uint4*)page)[e];
-        __syncthreads();
-        if (grown)
-            for (int e = threadIdx.x; e < it.tok0 * HD; e += NT) {
-                const int t = e / HD, c = e % HD;
-                uint8_t* pk = &s_img[0][kv_k_off(t, c, HD)];
-                uint8_t* pv = &s_img[1][kv_v_off(t, c)];
-                if (ks > old.x) *pk = (uint8_t)requant(*pk, old.x, ks, kr);
-                if (vs > old.y) *pv = (uint8_t)requant(*pv, old.y, vs, vr);
-            }
-    }
-#pragma unroll
-    for (int p = 0; p < PASSES; p++) {
-        const int i = first + 8 * p, tok = it.tok0 + i;
-        if (i >= it.n) continue;
-        *(uint16_t*)&s_img[0][kv_k_off(tok, d, HD)] = (uint16_t)(quant(x[p][0], ks, kr) | quant(x[p][1], ks, kr) << 8);
-        s_img[1][kv_v_off(tok, d)] = (uint8_t)quant(y[p][0], vs, vr);
-        s_img[1][kv_v_off(tok, d + 1)] = (uint8_t)quant(y[p][1], vs, vr);
-    }
-    __syncthreads();
-    // (positions behind the new rows are nobody's: what the image holds there goes along)
-    for (int e = threadIdx.x; e < 2 * PIECES; e += NT) ((uint4*)page)[e] = ((const uint4*)s_img)[e];
+    if (blockIdx.y == 0)
+        append_page<HD, false>(kv, it, head, rope, half, k, k_stride, bad, s_max, s_img);
+    else
+        append_page<HD, true>(kv, it, head, rope, half, v, v_stride, bad, s_max, s_img);
 }
 
-// One workgroup per (sequence, page of its last positions, KV head): the page's
-// bytes through LDS, four dimensions a thread on the way out.
+// One workgroup per (sequence, page of its last positions, KV head) and one of
+// keys and values: the page's bytes through LDS, four dimensions a thread on the
+// way out.
 template <int HD>
-__global__ __launch_bounds__(kBlock) void kv_read_kernel(KvView kv, KvPlanView p, int last, float* __restrict__ k_out,
+__global__ __launch_bounds__(HD * 4) void kv_read_kernel(KvView kv, KvPlanView p, int last, float* __restrict__ k_out,
                                                          float* __restrict__ v_out) {
-    constexpr int BYTES = kPage * HD, PIECES = BYTES / 16, Q = HD / 4;
-    __shared__ __attribute__((aligned(16))) uint8_t s_img[2][BYTES];
+    constexpr int NT = HD * 4, BYTES = kPage * HD, PIECES = BYTES / 16, Q = HD / 4;
+    __shared__ __attribute__((aligned(16))) uint8_t s_img[BYTES];
     __shared__ int s_row;
-    const int j = blockIdx.x / kv.kv_heads, head = blockIdx.x - j * kv.kv_heads, seq = blockIdx.y;
+    const int j = blockIdx.x / kv.kv_heads, head = blockIdx.x - j * kv.kv_heads, seq = blockIdx.y, which = blockIdx.z;
+    float* out = which ? v_out : k_out;
     const KvSeq s = p.seqs[seq];
     const int len = s.past + s.n_new, first = len > last ? len - last : 0;
     const int page = first / kPage + j;
-    if (page * kPage >= len) return;
+    if (!out || page * kPage >= len) return;
     const size_t cell = (size_t)p.pages[s.table0 + page] * kv.kv_heads + head;
-    const float2 scale = kv.scales[cell];
-    const uint4* from = (const uint4*)(kv.bytes + cell * 2 * BYTES);
-    for (int e = threadIdx.x; e < 2 * PIECES; e += kBlock) ((uint4*)s_img)[e] = from[e];
+    const float scale = which ? kv.scales[cell].y : kv.scales[cell].x;
+    const uint4* from = (const uint4*)(kv.bytes + (cell * 2 + which) * BYTES);
+    for (int e = threadIdx.x; e < PIECES; e += NT) ((uint4*)s_img)[e] = from[e];
     if (threadIdx.x == 0) s_row = 0;
     __syncthreads();
     // rows of the sequences before this one
     int before = 0;
-    for (int i = threadIdx.x; i < seq; i += kBlock) {
+    for (int i = threadIdx.x; i < seq; i += NT) {
         const int l = p.seqs[i].past + p.seqs[i].n_new;
         before += l < last ? l : last;
     }
     if (before) atomicAdd(&s_row, before);
     __syncthreads();
-    const size_t row0 = (size_t)s_row, width = (size_t)kv.kv_heads * HD;
+    const size_t width = (size_t)kv.kv_heads * HD;
+    out += ((size_t)s_row + page * kPage - first) * width + (size_t)head * HD;
     const int lo = max(first - page * kPage, 0), hi = min(len - page * kPage, kPage);
-    for (int e = lo * Q + threadIdx.x; e < hi * Q; e += kBlock) {
+    const bool vec = ((uintptr_t)out & 15) == 0;
+    for (int e = lo * Q + threadIdx.x; e < hi * Q; e += NT) {
         const int tok = e / Q, d = e % Q * 4;
-        const size_t o = (row0 + page * kPage + tok - first) * width + (size_t)head * HD + d;
-        const uint32_t kw = *(const uint32_t*)&s_img[0][kv_k_off(tok, d, HD)];
-        float a[4], b[4];
+        float w[4];
 #pragma unroll
-        for (int c = 0; c < 4; c++) {
-            a[c] = (float)((int)((kw >> (8 * c)) & 255u) - 128) * scale.x;
-            b[c] = (float)((int)s_img[1][kv_v_off(tok, d + c)] - 128) * scale.y;
+        for (int c = 0; c < 4; c++)
+            w[c] = (float)((int)s_img[which ? kv_v_off(tok, d + c) : kv_k_off(tok, d + c, HD)] - 128) * scale;
+        float* o = out + tok * width + d;
+        if (vec) {
+            *(float4*)o = make_float4(w[0], w[1], w[2], w[3]);
+        } else {
+#pragma unroll
+            for (int c = 0; c < 4; c++) o[c] = w[c];
         }
-        auto store = [](float* out, const float* w) {
-            if (((uintptr_t)out & 15) == 0) {
-                *(float4*)out = make_float4(w[0], w[1], w[2], w[3]);
-            } else {
-#pragma unroll
-                for (int c = 0; c < 4; c++) out[c] = w[c];
-            }
-        };
-        if (k_out) store(k_out + o, a);
-        if (v_out) store(v_out + o, b);
     }
 }
 
@@ -229,10 +231,10 @@ int launch_kv_append(hipStream_t s, const KvView& kv, const KvPlanView& p, const
     const size_t grid = (size_t)p.n_items * kv.kv_heads;
     if (grid > (size_t)INT32_MAX) return set_error(SQ_ERR_SHAPE, "kv_append: ShapeMismatch (too many pages)");
     if (kv.head_dim == 64)
-        hipLaunchKernelGGL(kv_append_kernel<64>, dim3((unsigned)grid), dim3(256), 0, s, kv, p.items, p.rope,
+        hipLaunchKernelGGL(kv_append_kernel<64>, dim3((unsigned)grid, 2), dim3(256), 0, s, kv, p.items, p.rope,
                            p.half, k, k_stride, v, v_stride, bad);
     else
-        hipLaunchKernelGGL(kv_append_kernel<128>, dim3((unsigned)grid), dim3(512), 0, s, kv, p.items, p.rope,
+        hipLaunchKernelGGL(kv_append_kernel<128>, dim3((unsigned)grid, 2), dim3(512), 0, s, kv, p.items, p.rope,
                            p.half, k, k_stride, v, v_stride, bad);
     return check_launch("kv_append");
 }
@@ -242,9 +244,9 @@ int launch_kv_read(hipStream_t s, const KvView& kv, const KvPlanView& p, int las
     const size_t grid = (size_t)max_pages * kv.kv_heads;
     if (grid > (size_t)INT32_MAX) return set_error(SQ_ERR_SHAPE, "kv_read: ShapeMismatch (too many pages)");
     if (kv.head_dim == 64)
-        hipLaunchKernelGGL(kv_read_kernel<64>, dim3((unsigned)grid, p.n_seqs), dim3(kBlock), 0, s, kv, p, last, k_out, v_out);
+        hipLaunchKernelGGL(kv_read_kernel<64>, dim3((unsigned)grid, p.n_seqs, 2), dim3(256), 0, s, kv, p, last, k_out, v_out);
     else
-        hipLaunchKernelGGL(kv_read_kernel<128>, dim3((unsigned)grid, p.n_seqs), dim3(kBlock), 0, s, kv, p, last, k_out, v_out);
+        hipLaunchKernelGGL(kv_read_kernel<128>, dim3((unsigned)grid, p.n_seqs, 2), dim3(512), 0, s, kv, p, last, k_out, v_out);
     return check_launch("kv_read");
 }
 
