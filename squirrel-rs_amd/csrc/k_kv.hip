@@ -21,13 +21,15 @@ inline int check_launch(const char* what) {
 }
 
 __global__ __launch_bounds__(64) void kv_rope_kernel(const KvSeq* __restrict__ seqs, int half,
-                                                     const float* __restrict__ inv_freq, double2* __restrict__ out) {
+                                                     const float* __restrict__ inv_freq, double2* __restrict__ out,
+                                                     float2* __restrict__ out32) {
     const KvSeq s = seqs[blockIdx.y];
     for (int i = blockIdx.x; i < s.n_new; i += gridDim.x)
         for (int j = threadIdx.x; j < half; j += 64) {
             double sn, cs;
             sincos((double)(s.past + i) * (double)inv_freq[j], &sn, &cs);
             out[(size_t)(s.row0 + i) * half + j] = double2{cs, sn};
+            out32[(size_t)(s.row0 + i) * half + j] = make_float2((float)cs, (float)sn);
         }
 }
 
@@ -220,9 +222,9 @@ __global__ __launch_bounds__(HD * 4) void kv_read_kernel(KvView kv, KvPlanView p
 
 }  // namespace
 
-int launch_kv_rope(hipStream_t s, const KvPlanView& p, const float* inv_freq, int rows, double2* out) {
+int launch_kv_rope(hipStream_t s, const KvPlanView& p, const float* inv_freq, int rows, double2* out, float2* out32) {
     hipLaunchKernelGGL(kv_rope_kernel, dim3(std::min(rows, 1024), p.n_seqs), dim3(64), 0, s, p.seqs, p.half, inv_freq,
-                       out);
+                       out, out32);
     return check_launch("kv_rope");
 }
 

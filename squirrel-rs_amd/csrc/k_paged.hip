@@ -86,20 +86,15 @@ __device__ __forceinline__ v8h unpack8(uint32_t a, uint32_t b) {
     return r;
 }
 
-// Maximum / sum over the four lanes that share a query (l % 16).
+// Maximum over the four lanes that share a query (l % 16).
 __device__ __forceinline__ float groups_max(float v) {
     v = fmaxf(v, __shfl_xor(v, 16, 64));
     return fmaxf(v, __shfl_xor(v, 32, 64));
 }
-__device__ __forceinline__ float groups_sum(float v) {
-    v += __shfl_xor(v, 16, 64);
-    return v + __shfl_xor(v, 32, 64);
-}
-
 // E consecutive dimensions of one query row from `d`, rotated; false where one
 // is not finite.
 template <int E>
-__device__ __forceinline__ bool load_query(const float* q, bool vec, const double2* rope, int half, int d, float* x) {
+__device__ __forceinline__ bool load_query(const float* q, bool vec, const float2* rope, int half, int d, float* x) {
     if (vec) {
 #pragma unroll
         for (int e = 0; e < E; e += 4) {
@@ -117,11 +112,11 @@ __device__ __forceinline__ bool load_query(const float* q, bool vec, const doubl
 #pragma unroll
         for (int e = 0; e < E; e += 2) {
             const int j = (d + e) / 2;
-            const double2 cs = rope[min(j, half - 1)];
-            const double u = x[e], v = x[e + 1];
+            const float2 cs = rope[min(j, half - 1)];
+            const float u = x[e], v = x[e + 1];
             if (j < half) {
-                x[e] = (float)(u * cs.x - v * cs.y);
-                x[e + 1] = (float)(u * cs.y + v * cs.x);
+                x[e] = u * cs.x - v * cs.y;
+                x[e + 1] = u * cs.y + v * cs.x;
             }
         }
     }
@@ -167,16 +162,20 @@ constexpr int kStat = 4;  // floats behind a part's sums: the maximum, the sum o
 constexpr float kBase = 8.0f, kHeadroom = 6.0f;
 constexpr float kSmall = 0x1p-8f;  // of the sums' unit: the scales of a page's values that need no other
 template <int HD, int R, int NW, bool PAGES>
-__global__ __launch_bounds__(NW * 64, PAGES ? (HD == 64 ? 3 : 2) : 2) void sdpa_paged_kernel(KvView kv, KvPlanView pl, PagedArgs a, Cut cut, float scale) {
+__global__ __launch_bounds__(NW * 64, PAGES ? (HD == 64 ? 3 : 2) : (HD == 64 ? 4 : 2)) void sdpa_paged_kernel(KvView kv, KvPlanView pl, PagedArgs a, Cut cut, float scale) {
     constexpr int C = HD / 64, DT = HD / 16, TR = PAGES ? 16 * R : NW * 16 * R;
     __shared__ __attribute__((aligned(16))) float s_o[PAGES ? NW * 16 * R * (HD + 4) : 1];
     __shared__ __attribute__((aligned(16))) _Float16 s_q[2][PAGES ? 16 * R * HD : 8];
     __shared__ float s_cq[PAGES ? 16 * R : 1];
+    __shared__ __attribute__((aligned(16))) v8h s_kv[PAGES ? 1 : 2][PAGES ? 1 : 16 * C * 64];
     __shared__ float s_m[PAGES ? NW * 16 * R : 1], s_l[PAGES ? NW * 16 * R : 1];
     // (heads next to each other: with eight of them each is one XCD's, and a
-    // head's tiles share that XCD's L2; a sequence's last tiles, which see the most
-    // pages, first)
-    const int at = cut.by_heads(blockIdx.x), head = blockIdx.x - at * kv.kv_heads, tile = cut.tiles - 1 - at;
+    // head's tiles share that XCD's L2.  A sequence's last tiles see the most pages:
+    // they come first, and every second 32 of a head's, one for each CU of an XCD,
+    // in the other order, so that the CUs' shares are alike)
+    const int at = cut.by_heads(blockIdx.x), head = blockIdx.x - at * kv.kv_heads;
+    const int from = at & ~31, turned = (at & 32) ? from + min(cut.tiles, from + 32) - 1 - at : at;
+    const int tile = cut.tiles - 1 - turned;
     const int part = blockIdx.y, seq = blockIdx.z;
     const KvSeq s = pl.seqs[seq];
     const int G = (int)cut.by_group.d, rows = s.n_new * G;
@@ -191,33 +190,45 @@ __global__ __launch_bounds__(NW * 64, PAGES ? (HD == 64 ? 3 : 2) : 2) void sdpa_
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, q16 = lane & 15, g = lane >> 4;
     const int row0 = tile * TR + (PAGES ? 0 : wave * 16 * R);  // the wavefront's first row
 
-    // The bytes of one page in registers: keys, then values.  A page's keys are
-    // requested before the second product of the page before, its values
-    // behind it.
+    // A page's bytes are 8 C pieces of 1 KB, one load of a wavefront each: keys,
+    // then values.
+    // PAGES: the wavefront's page in registers; the next one's keys are requested
+    // before the second product, its values behind it.
+    // Otherwise the wavefronts share the work on a page: each loads and unpacks
+    // its pieces of the page after next into one of two f16 images in LDS.
+    // (Unpacked by every wavefront for itself that was 128 of 286 VALU
+    // instructions for 16 rows of a page: 62 us against 4x for a prompt's 1531 rows.)
+    constexpr int P = 8 * C, OWN = PAGES ? P : P / NW;
+    static_assert(PAGES || P % NW == 0, "whole pieces a wavefront");
     const int step = PAGES ? NW : 1;
     int i = part * cut.chunk + (PAGES ? wave : 0);
-    uint4 kw[4][C], vw[DT];
+    uint4 w[OWN];
     float2 sc = make_float2(0.0f, 0.0f), sc_next = sc;
     const uint4* kb = nullptr;
-    auto locate = [&](int i) {
-        const size_t cell = (size_t)pl.pages[s.table0 + span.page(i)] * kv.kv_heads + head;
+    // (a page's number is asked for an iteration before its bytes)
+    auto number = [&](int i) { return pl.pages[s.table0 + span.page(min(i, i_end - 1))]; };
+    auto locate = [&](int id) {
+        const size_t cell = (size_t)id * kv.kv_heads + head;
         sc_next = kv.scales[cell];
-        kb = (const uint4*)(kv.bytes + cell * 2 * kPage * HD) + lane;
+        kb = (const uint4*)(kv.bytes + cell * 2 * kPage * HD) + lane + (PAGES ? 0 : wave * OWN * 64);
     };
-    auto load_keys = [&] {
+    auto load = [&](int from, int to) {
 #pragma unroll
-        for (int t = 0; t < 4; t++)
-#pragma unroll
-            for (int c = 0; c < C; c++) kw[t][c] = kb[(t * C + c) * 64];
+        for (int e = from; e < to; e++) w[e] = kb[e * 64];
     };
-    auto load_values = [&] {
+    auto share = [&](int buffer) {
 #pragma unroll
-        for (int d = 0; d < DT; d++) vw[d] = kb[(4 * C + d) * 64];
+        for (int e = 0; e < OWN; e++) {
+            v8h* to = &s_kv[buffer][((wave * OWN + e) * 2) * 64 + lane];
+            to[0] = unpack8(w[e].x, w[e].y);
+            to[64] = unpack8(w[e].z, w[e].w);
+        }
     };
+    const int id0 = number(i);
+    int id = number(i + step);
     if (i < i_end) {
-        locate(i);
-        load_keys();
-        load_values();
+        locate(id0);
+        load(0, OWN);
     }
 
     // Queries: [chunk of 64][half of a lane's 16 dimensions].
@@ -229,7 +240,7 @@ __global__ __launch_bounds__(NW * 64, PAGES ? (HD == 64 ? 3 : 2) : 2) void sdpa_
         const int i = cut.by_group(r);
         return a.q + ((size_t)s.row0 + i) * a.q_stride + (size_t)(head * G + r - i * G) * HD;
     };
-    auto rope = [&](int r) { return pl.rope ? pl.rope + ((size_t)s.row0 + cut.by_group(r)) * pl.half : nullptr; };
+    auto rope = [&](int r) { return pl.rope32 ? pl.rope32 + ((size_t)s.row0 + cut.by_group(r)) * pl.half : nullptr; };
 #pragma unroll
     for (int u = 0; u < R; u++) {
         const int r = min(row0 + 16 * u + q16, rows - 1);
@@ -299,6 +310,8 @@ __global__ __launch_bounds__(NW * 64, PAGES ? (HD == 64 ? 3 : 2) : 2) void sdpa_
 
     // (-1 that the compiler does not know to be: p - h then takes the f16 half as it
     // is, where it would convert it to f32 first)
+    const v8h ones = {(_Float16)1.0f, (_Float16)1.0f, (_Float16)1.0f, (_Float16)1.0f,
+                      (_Float16)1.0f, (_Float16)1.0f, (_Float16)1.0f, (_Float16)1.0f};
     float minus = -1.0f;
     asm volatile("" : "+v"(minus));
     v4f o[R][DT];
@@ -313,9 +326,32 @@ __global__ __launch_bounds__(NW * 64, PAGES ? (HD == 64 ? 3 : 2) : 2) void sdpa_
     const int pos_lo = s.past + cut.by_group(row0), pos_hi = s.past + cut.by_group(min(rows, row0 + 16 * R) - 1);
     const int w0_hi = a.window && a.window <= pos_hi ? pos_hi - a.window + 1 : 0;
 
+    int turn = 0;
+    if constexpr (!PAGES) {  // (a launch's parts are never empty)
+        share(0);
+        sc = sc_next;
+        if (i + 1 < i_end) {
+            locate(id);
+            load(0, OWN);
+            id = number(i + 2);
+        }
+        __syncthreads();
+    }
     for (; i < i_end; i += step) {
         const int page = span.page(i);
-        sc = sc_next;
+        const bool more = i + step < i_end;
+        if constexpr (PAGES) {
+            sc = sc_next;
+        } else if (more) {
+            share(turn ^ 1);
+        }
+        // half h of piece e
+        auto half = [&](int e, int h) {
+            if constexpr (PAGES)
+                return h ? unpack8(w[e].z, w[e].w) : unpack8(w[e].x, w[e].y);
+            else
+                return s_kv[turn][(e * 2 + h) * 64 + lane];
+        };
         // scores [tile of 16 positions][position 4 g + r]
         v4f x[R][4];
 #pragma unroll
@@ -324,7 +360,7 @@ __global__ __launch_bounds__(NW * 64, PAGES ? (HD == 64 ? 3 : 2) : 2) void sdpa_
             for (int u = 0; u < R; u++) x[u][t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int c = 0; c < C; c++) {
-                const v8h k0 = unpack8(kw[t][c].x, kw[t][c].y), k1 = unpack8(kw[t][c].z, kw[t][c].w);
+                const v8h k0 = half(t * C + c, 0), k1 = half(t * C + c, 1);
 #pragma unroll
                 for (int u = 0; u < R; u++) {
                     x[u][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, ql[u][c][0], x[u][t], 0, 0, 0);
@@ -370,9 +406,9 @@ __global__ __launch_bounds__(NW * 64, PAGES ? (HD == 64 ? 3 : 2) : 2) void sdpa_
             for (int t = 0; t < 4; t++)
 #pragma unroll
                 for (int r = 0; r < 4; r++) mx = fmaxf(mx, x[u][t][r]);
-            mx = groups_max(mx * cs);
+            mx *= cs;
             if (__any(mx > m[u] + kHeadroom)) {
-                const float mn = fmaxf(m[u], mx);
+                const float mn = fmaxf(m[u], groups_max(mx));
                 const float alpha = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[u] - mn);
                 m[u] = mn;
                 l[u] *= alpha;
@@ -380,14 +416,12 @@ __global__ __launch_bounds__(NW * 64, PAGES ? (HD == 64 ? 3 : 2) : 2) void sdpa_
                 for (int d = 0; d < DT; d++) o[u][d] *= alpha;
             }
             const float off = kBase - (m[u] == -INFINITY ? 0.0f : m[u]) + lr;
-            float sum = 0.0f;
 #pragma unroll
             for (int r = 0; r < 4; r++)
 #pragma unroll
                 for (int t = 0; t < 4; t += 2) {
                     const v2f p = {__builtin_amdgcn_exp2f(fmaf(x[u][t][r], cs, off)),
                                    __builtin_amdgcn_exp2f(fmaf(x[u][t + 1][r], cs, off))};
-                    sum += p[0] + p[1];
                     const v2h h = __builtin_convertvector(p, v2h);
                     const v2f rest = {fmaf((float)h[0], minus, p[0]), fmaf((float)h[1], minus, p[1])};
                     const v2h w = __builtin_convertvector(rest, v2h);
@@ -395,12 +429,18 @@ __global__ __launch_bounds__(NW * 64, PAGES ? (HD == 64 ? 3 : 2) : 2) void sdpa_
                     ph[u][j / 8][j % 8] = h[0], ph[u][j / 8][j % 8 + 1] = h[1];
                     plo[u][j / 8][j % 8] = w[0], plo[u][j / 8][j % 8 + 1] = w[1];
                 }
-            l[u] += sum * back;
+            // the weights' sum on the matrix pipe, of the halves as they are used
+            v4f sum = {0.0f, 0.0f, 0.0f, 0.0f};
+            sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, plo[u][0], sum, 0, 0, 0);
+            sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, plo[u][1], sum, 0, 0, 0);
+            sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, ph[u][0], sum, 0, 0, 0);
+            sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, ph[u][1], sum, 0, 0, 0);
+            l[u] += sum[0] * back;
         }
-        const bool more = i + step < i_end;
-        if (more) {
-            locate(i + step);
-            load_keys();
+        if (PAGES && more) {
+            locate(id);
+            load(0, 4 * C);
+            id = number(i + 2 * step);
         }
         auto weigh = [&](int u, v8h v0, v8h v1, v4f y) {
             y = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, plo[u][0], y, 0, 0, 0);
@@ -410,18 +450,27 @@ __global__ __launch_bounds__(NW * 64, PAGES ? (HD == 64 ? 3 : 2) : 2) void sdpa_
         };
 #pragma unroll
         for (int d = 0; d < DT; d++) {
-            const v8h v0 = unpack8(vw[d].x, vw[d].y), v1 = unpack8(vw[d].z, vw[d].w);
+            const v8h v0 = half(4 * C + d, 0), v1 = half(4 * C + d, 1);
 #pragma unroll
             for (int u = 0; u < R; u++) o[u][d] = weigh(u, v0, v1, o[u][d]);
         }
-        if (more) load_values();
+        if constexpr (PAGES) {
+            if (more) load(4 * C, P);
+        } else {
+            sc = sc_next;
+            if (i + 2 < i_end) {
+                locate(id);
+                load(0, OWN);
+                id = number(i + 3);
+            }
+            turn ^= 1;
+            __syncthreads();
+        }
     }
 #pragma unroll
     for (int u = 0; u < R; u++)
 #pragma unroll
         for (int d = 0; d < DT; d++) o[u][d] *= vref;
-#pragma unroll
-    for (int u = 0; u < R; u++) l[u] = groups_sum(l[u]);
 
     // where four of row r's sums go: its output, or its part of the workspace
     const bool vec_out = (((uintptr_t)a.out | (a.out_stride * 4)) & 15) == 0;
@@ -546,7 +595,7 @@ __global__ __launch_bounds__(256) void sdpa_merge_kernel(KvView kv, KvPlanView p
 
 // Sequences of few rows: wavefronts over pages, tiles of 16 rows; of more: wavefronts over
 // rows, tiles of 128 (of 64 with 128 dimensions, whose sums take the registers of two).
-constexpr int kFewWaves = 4, kFewRows = 64, kTileFew = 16, kTileMany = 128;
+constexpr int kFewWaves = 4, kFewRows = 64, kTileFew = 16, kTileMany = 64;
 constexpr int kTarget = 512, kTargetMany = 512;  // workgroups that a launch is cut into
 
 struct Launch {
@@ -555,7 +604,7 @@ struct Launch {
     bool any;
 };
 Launch plan_launch(const std::vector<KvSeq>& seqs, const KvView& kv, const PagedArgs& a, bool many) {
-    const int G = a.heads / kv.kv_heads, tile = !many ? kTileFew : kv.head_dim == 64 ? kTileMany : kTileMany / 2;
+    const int G = a.heads / kv.kv_heads, tile = !many ? kTileFew : kTileMany;
     Launch r{};
     r.cut.rows_lo = many ? kFewRows + 1 : 1;
     r.cut.by_group = Div(G);
@@ -626,7 +675,7 @@ int launch_sdpa_paged(hipStream_t s, const std::vector<KvSeq>& seqs, const KvVie
         l.cut.ws = ws;
         int st;
         if (kv.head_dim == 64)
-            st = many ? launch_one<64, 2, 4, false>(s, l, kv, p, a) : launch_one<64, 1, kFewWaves, true>(s, l, kv, p, a);
+            st = many ? launch_one<64, 1, 4, false>(s, l, kv, p, a) : launch_one<64, 1, kFewWaves, true>(s, l, kv, p, a);
         else
             st = many ? launch_one<128, 1, 4, false>(s, l, kv, p, a) : launch_one<128, 1, kFewWaves, true>(s, l, kv, p, a);
         if (st) return st;

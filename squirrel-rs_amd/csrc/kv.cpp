@@ -205,6 +205,7 @@ int kv_views(sq_kv_plan* plan, size_t layer, bool rotate, const char* what, KvVi
                      (const int*)(plan->dev + plan->off_pages),
                      (const KvItem*)(plan->dev + plan->off_items),
                      nullptr,
+                     nullptr,
                      (int)plan->seqs.size(),
                      (int)plan->n_items,
                      (int)plan->rows,
@@ -212,11 +213,14 @@ int kv_views(sq_kv_plan* plan, size_t layer, bool rotate, const char* what, KvVi
     if (!rotate || !pool.half || !plan->rows) return 0;
     if (!plan->rope_ready) {
         // (growing frees nothing that a queued launch reads: every call waits for its own)
-        if (int st = grow((void**)&plan->rope, &plan->rope_size, plan->rows * pool.half * sizeof(double2))) return st;
-        if (int st = launch_kv_rope(nullptr, *pv, pool.inv_freq, (int)plan->rows, plan->rope)) return st;
+        const size_t n = plan->rows * pool.half;
+        if (int st = grow((void**)&plan->rope, &plan->rope_size, n * (sizeof(double2) + sizeof(float2)))) return st;
+        if (int st = launch_kv_rope(nullptr, *pv, pool.inv_freq, (int)plan->rows, plan->rope, (float2*)(plan->rope + n)))
+            return st;
         plan->rope_ready = true;
     }
     pv->rope = plan->rope;
+    pv->rope32 = (const float2*)(plan->rope + plan->rows * pool.half);
     return 0;
 }
 

@@ -61,12 +61,13 @@ struct KvPlanView {
     const KvSeq* seqs;
     const int* pages;
     const KvItem* items;
-    const double2* rope;  // [rows][half] (cos, sin), null: nothing is rotated
+    const double2* rope;   // [rows][half] (cos, sin), null: nothing is rotated
+    const float2* rope32;  // the same in f32: queries, which no integer is decided by
     int n_seqs, n_items, rows, half;
 };
 
 // ---- k_kv.hip
-int launch_kv_rope(hipStream_t s, const KvPlanView& p, const float* inv_freq, int rows, double2* out);
+int launch_kv_rope(hipStream_t s, const KvPlanView& p, const float* inv_freq, int rows, double2* out, float2* out32);
 int launch_kv_append(hipStream_t s, const KvView& kv, const KvPlanView& p, const float* k, size_t k_stride,
                      const float* v, size_t v_stride, uint32_t* bad);
 // max_pages: the most pages that a sequence's last `last` positions lie in.
@@ -103,7 +104,7 @@ struct sq_kv_plan {
     uint8_t* dev = nullptr;  // seqs, items, pages
     size_t dev_size = 0;
     size_t off_items = 0, off_pages = 0;
-    double2* rope = nullptr;  // made by the first call that rotates
+    double2* rope = nullptr;  // [rows][half], then the same in f32; made by the first call that rotates
     size_t rope_size = 0;
     bool rope_ready = false;
     uint32_t* bad = nullptr;  // pinned: set by a kernel that met a value which is not finite
