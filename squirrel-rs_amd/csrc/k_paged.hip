@@ -86,11 +86,24 @@ __device__ __forceinline__ v8h unpack8(uint32_t a, uint32_t b) {
     return r;
 }
 
-// Maximum over the four lanes that share a query (l % 16).
+// Maximum / sum over the four lanes that share a query (l % 16).
 __device__ __forceinline__ float groups_max(float v) {
     v = fmaxf(v, __shfl_xor(v, 16, 64));
     return fmaxf(v, __shfl_xor(v, 32, 64));
 }
+__device__ __forceinline__ float groups_sum(float v) {
+    v += __shfl_xor(v, 16, 64);
+    return v + __shfl_xor(v, 32, 64);
+}
+
+// Scales of a sequence's pages are taken relative to its first page's (1 where
+// that holds zeros), within 2^96 of it either way: their quotients stay in f32.
+// A page of zeros may have any scale.
+__device__ __forceinline__ float first_unit(float scale) { return scale > 0.0f ? fminf(fmaxf(scale, 0x1p-30f), 0x1p30f) : 1.0f; }
+__device__ __forceinline__ float page_unit(float scale, float unit) {
+    return scale > 0.0f ? fminf(fmaxf(scale, unit * 0x1p-96f), unit * 0x1p96f) : unit;
+}
+
 // E consecutive dimensions of one query row from `d`, rotated; false where one
 // is not finite.
 template <int E>
@@ -151,16 +164,18 @@ __device__ __forceinline__ void halves(float x, int shift, _Float16& h, _Float16
 // two f16 halves each (x = hi + lo to 2^-22 of x): two products on the matrix
 // pipe give what one in f32 would, four times as fast.
 //
-// A row's maximum follows its scores in steps: as long as they stay within
-// kHeadroom of it (in powers of two) nothing is rescaled, and the weights
-// stay below 2^(kBase + kHeadroom + 1) = 2^15, in f16's range with kBase bits
-// of room for the small ones.
+// A weight w_j = 2^(score_j) comes with its page's value scale: the second
+// product's operand is w_j v_scale and the sum of weights takes w_j v_scale *
+// (unit / v_scale) in f32.  So the matrix pipe adds to the sums in place, and it is
+// the products that count, not the weights, that keep their 22 bits.
+// A row's maximum (of score + log2 v_scale) follows in steps: as long as they
+// stay within kHeadroom of it nothing is rescaled, and the operands stay below
+// 2^(kBase + kHeadroom), in f16's range with kBase bits of room for small ones.
 //
 // PAGES: the wavefronts take pages in turn for the same 16 R rows and meet in
 // LDS; otherwise each has its own 16 R rows and all walk the same pages.
 constexpr int kStat = 4;  // floats behind a part's sums: the maximum, the sum of weights, two unused
 constexpr float kBase = 8.0f, kHeadroom = 6.0f;
-constexpr float kSmall = 0x1p-8f;  // of the sums' unit: the scales of a page's values that need no other
 template <int HD, int R, int NW, bool PAGES>
 __global__ __launch_bounds__(NW * 64, PAGES ? (HD == 64 ? 3 : 2) : (HD == 64 ? 4 : 2)) void sdpa_paged_kernel(KvView kv, KvPlanView pl, PagedArgs a, Cut cut, float scale) {
     constexpr int C = HD / 64, DT = HD / 16, TR = PAGES ? 16 * R : NW * 16 * R;
@@ -230,6 +245,8 @@ __global__ __launch_bounds__(NW * 64, PAGES ? (HD == 64 ? 3 : 2) : (HD == 64 ? 4
         locate(id0);
         load(0, OWN);
     }
+
+    const float unit = first_unit(kv.scales[(size_t)pl.pages[s.table0] * kv.kv_heads + head].y);
 
     // Queries: [chunk of 64][half of a lane's 16 dimensions].
     v8h qh[R][C][2], ql[R][C][2];
@@ -310,12 +327,10 @@ __global__ __launch_bounds__(NW * 64, PAGES ? (HD == 64 ? 3 : 2) : (HD == 64 ? 4
 
     // (-1 that the compiler does not know to be: p - h then takes the f16 half as it
     // is, where it would convert it to f32 first)
-    const v8h ones = {(_Float16)1.0f, (_Float16)1.0f, (_Float16)1.0f, (_Float16)1.0f,
-                      (_Float16)1.0f, (_Float16)1.0f, (_Float16)1.0f, (_Float16)1.0f};
     float minus = -1.0f;
     asm volatile("" : "+v"(minus));
     v4f o[R][DT];
-    float m[R], l[R], vref = 0.0f, vtop = 0.0f;
+    float m[R], l[R];
 #pragma unroll
     for (int t = 0; t < R; t++) {
         m[t] = -INFINITY, l[t] = 0.0f;
@@ -371,21 +386,7 @@ __global__ __launch_bounds__(NW * 64, PAGES ? (HD == 64 ? 3 : 2) : (HD == 64 ? 4
             }
         }
         const bool full = (page + 1) * kPage - 1 <= pos_lo && (page * kPage >= w0_hi || (page + 1) * kPage <= a.sinks);
-        // The sums stand in units of vref, near the scale of the page's values; a
-        // page's weights carry the rest of it, so that the matrix pipe adds to the
-        // sums in place.  (The unit goes no further than 2^-64 below the largest
-        // so far: the sums stay in range, and what that costs is 2^-70 of those
-        // values.  A page of zeros adds nothing in any unit.)
-        if (sc.y > 0.0f && !(sc.y <= 2.0f * vref && sc.y >= kSmall * vref)) {
-            vtop = fmaxf(vtop, sc.y);
-            const float to = fmaxf(sc.y, 0x1p-64f * vtop), f = vref > 0.0f ? vref / to : 0.0f;
-#pragma unroll
-            for (int u = 0; u < R; u++)
-#pragma unroll
-                for (int d = 0; d < DT; d++) o[u][d] *= f;
-            vref = to;
-        }
-        const float lr = sc.y > 0.0f ? __builtin_amdgcn_logf(sc.y / vref) : 0.0f, back = __builtin_amdgcn_exp2f(-lr);
+        const float vs = page_unit(sc.y, unit), lr = __builtin_amdgcn_logf(vs), back = unit / vs;
         v8h ph[R][2], plo[R][2];
 #pragma unroll
         for (int u = 0; u < R; u++) {
@@ -406,7 +407,7 @@ __global__ __launch_bounds__(NW * 64, PAGES ? (HD == 64 ? 3 : 2) : (HD == 64 ? 4
             for (int t = 0; t < 4; t++)
 #pragma unroll
                 for (int r = 0; r < 4; r++) mx = fmaxf(mx, x[u][t][r]);
-            mx *= cs;
+            mx = mx * cs + lr;
             if (__any(mx > m[u] + kHeadroom)) {
                 const float mn = fmaxf(m[u], groups_max(mx));
                 const float alpha = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[u] - mn);
@@ -416,12 +417,14 @@ __global__ __launch_bounds__(NW * 64, PAGES ? (HD == 64 ? 3 : 2) : (HD == 64 ? 4
                 for (int d = 0; d < DT; d++) o[u][d] *= alpha;
             }
             const float off = kBase - (m[u] == -INFINITY ? 0.0f : m[u]) + lr;
+            float sum = 0.0f;
 #pragma unroll
             for (int r = 0; r < 4; r++)
 #pragma unroll
                 for (int t = 0; t < 4; t += 2) {
                     const v2f p = {__builtin_amdgcn_exp2f(fmaf(x[u][t][r], cs, off)),
                                    __builtin_amdgcn_exp2f(fmaf(x[u][t + 1][r], cs, off))};
+                    sum += p[0] + p[1];
                     const v2h h = __builtin_convertvector(p, v2h);
                     const v2f rest = {fmaf((float)h[0], minus, p[0]), fmaf((float)h[1], minus, p[1])};
                     const v2h w = __builtin_convertvector(rest, v2h);
@@ -429,13 +432,7 @@ __global__ __launch_bounds__(NW * 64, PAGES ? (HD == 64 ? 3 : 2) : (HD == 64 ? 4
                     ph[u][j / 8][j % 8] = h[0], ph[u][j / 8][j % 8 + 1] = h[1];
                     plo[u][j / 8][j % 8] = w[0], plo[u][j / 8][j % 8 + 1] = w[1];
                 }
-            // the weights' sum on the matrix pipe, of the halves as they are used
-            v4f sum = {0.0f, 0.0f, 0.0f, 0.0f};
-            sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, plo[u][0], sum, 0, 0, 0);
-            sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, plo[u][1], sum, 0, 0, 0);
-            sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, ph[u][0], sum, 0, 0, 0);
-            sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, ph[u][1], sum, 0, 0, 0);
-            l[u] += sum[0] * back;
+            l[u] += sum * back;
         }
         if (PAGES && more) {
             locate(id);
@@ -468,9 +465,7 @@ __global__ __launch_bounds__(NW * 64, PAGES ? (HD == 64 ? 3 : 2) : (HD == 64 ? 4
         }
     }
 #pragma unroll
-    for (int u = 0; u < R; u++)
-#pragma unroll
-        for (int d = 0; d < DT; d++) o[u][d] *= vref;
+    for (int u = 0; u < R; u++) l[u] = groups_sum(l[u]);
 
     // where four of row r's sums go: its output, or its part of the workspace
     const bool vec_out = (((uintptr_t)a.out | (a.out_stride * 4)) & 15) == 0;
@@ -478,7 +473,7 @@ __global__ __launch_bounds__(NW * 64, PAGES ? (HD == 64 ? 3 : 2) : (HD == 64 ? 4
         if (whole) {
             const int i = cut.by_group(r);
             float* out = a.out + ((size_t)s.row0 + i) * a.out_stride + (size_t)(head * G + r - i * G) * HD + d;
-            v *= 1.0f / ll;
+            v *= unit / ll;
             if (vec_out) {
                 *(v4f*)out = v;
             } else {
@@ -533,22 +528,28 @@ __global__ __launch_bounds__(NW * 64, PAGES ? (HD == 64 ? 3 : 2) : (HD == 64 ? 4
     }
 }
 
-// The parts of the rows whose pages were cut: one workgroup per (sequence, KV
-// head, row).  A wavefront's lanes find the factors of 64 parts, then it adds
-// every fourth part, eight in flight at a time.
-template <int HD>
+// The parts of the rows whose pages were cut, from (sequence, KV head, row).
+// W wavefronts share a row: all four of a workgroup where rows are few and parts
+// many (131000 positions: 32 rows of 21 parts), one where it is the other way.
+// The lanes find the factors of 64 parts, then a wavefront adds every W-th
+// part, eight in flight at a time.
+template <int HD, int W>
 __global__ __launch_bounds__(256) void sdpa_merge_kernel(KvView kv, KvPlanView pl, PagedArgs a, Cut cut, int tile_rows) {
     constexpr int C = HD / 64, IN = 8;
     __shared__ float s_o[4][HD];
-    const int seq = blockIdx.y, r = cut.by_heads(blockIdx.x), head = blockIdx.x - r * kv.kv_heads;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, mine = wave % W;
+    const int seq = blockIdx.y, at = cut.by_heads(blockIdx.x), head = blockIdx.x - at * kv.kv_heads;
+    const int r = at * (4 / W) + wave / W;
     const KvSeq s = pl.seqs[seq];
     const int G = (int)cut.by_group.d, rows = s.n_new * G;
-    if (rows < cut.rows_lo || rows > cut.rows_hi || r >= rows) return;
-    const int tile = r / tile_rows, row_end = min(rows, (tile + 1) * tile_rows);
-    const Span span = tile_span(s.past + cut.by_group(tile * tile_rows), s.past + cut.by_group(row_end - 1), a.window, a.sinks);
-    const int parts = cut.parts(span.count);
-    if (parts == 1) return;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
+    int parts = 1;
+    if (rows >= cut.rows_lo && rows <= cut.rows_hi && r < rows) {
+        const int tile = r / tile_rows, row_end = min(rows, (tile + 1) * tile_rows);
+        const Span span = tile_span(s.past + cut.by_group(tile * tile_rows), s.past + cut.by_group(row_end - 1), a.window, a.sinks);
+        parts = cut.parts(span.count);
+    }
+    if (parts == 1) return;  // (W = 4: the whole workgroup)
+    const float unit = first_unit(kv.scales[(size_t)pl.pages[s.table0] * kv.kv_heads + head].y);
     const size_t stride = (size_t)kv.kv_heads * cut.rows_hi * (HD + kStat);
     const float* w = cut.ws + ((cut.slot(s, seq, 0) * kv.kv_heads + head) * cut.rows_hi + r) * (HD + kStat);
     float mm = -INFINITY, ll = 0.0f, o[C] = {};
@@ -563,40 +564,44 @@ __global__ __launch_bounds__(256) void sdpa_merge_kernel(KvView kv, KvPlanView p
             ll += l1 * f;
         }
         const int n = min(parts - i0, 64);
-        for (int k = wave; k < n; k += 4 * IN) {
+        for (int k = mine; k < n; k += W * IN) {
             float v[IN][C];
 #pragma unroll
             for (int j = 0; j < IN; j++)
 #pragma unroll
-                for (int c = 0; c < C; c++) v[j][c] = w[(i0 + min(k + 4 * j, n - 1)) * stride + 64 * c + lane];
+                for (int c = 0; c < C; c++) v[j][c] = k + W * j < n ? w[(i0 + k + W * j) * stride + 64 * c + lane] : 0.0f;
 #pragma unroll
             for (int j = 0; j < IN; j++) {
                 const float fj = __builtin_bit_cast(
-                    float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), min(k + 4 * j, 63)));
-                if (k + 4 * j < n)
+                    float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), min(k + W * j, 63)));
+                if (k + W * j < n)
 #pragma unroll
                     for (int c = 0; c < C; c++) o[c] += v[j][c] * fj;
             }
         }
     }
     ll = sq_wave_sum(ll);
+    if constexpr (W > 1) {
 #pragma unroll
-    for (int c = 0; c < C; c++) s_o[wave][64 * c + lane] = o[c];
-    __syncthreads();
-    if (wave) return;
+        for (int c = 0; c < C; c++) s_o[wave][64 * c + lane] = o[c];
+        __syncthreads();
+        if (wave) return;
+#pragma unroll
+        for (int c = 0; c < C; c++) {
+            const int d = 64 * c + lane;
+            o[c] = (s_o[0][d] + s_o[1][d]) + (s_o[2][d] + s_o[3][d]);
+        }
+    }
     const int i = cut.by_group(r);
     float* out = a.out + ((size_t)s.row0 + i) * a.out_stride + (size_t)(head * G + r - i * G) * HD;
 #pragma unroll
-    for (int c = 0; c < C; c++) {
-        const int d = 64 * c + lane;
-        out[d] = ((s_o[0][d] + s_o[1][d]) + (s_o[2][d] + s_o[3][d])) / ll;
-    }
+    for (int c = 0; c < C; c++) out[64 * c + lane] = o[c] * (unit / ll);
 }
 
 // Sequences of few rows: wavefronts over pages, tiles of 16 rows; of more: wavefronts over
 // rows, tiles of 128 (of 64 with 128 dimensions, whose sums take the registers of two).
 constexpr int kFewWaves = 4, kFewRows = 64, kTileFew = 16, kTileMany = 64;
-constexpr int kTarget = 512, kTargetMany = 512;  // workgroups that a launch is cut into
+constexpr int kTarget = 768, kTargetMany = 512;  // workgroups that a launch is cut into
 
 struct Launch {
     Cut cut;
@@ -630,7 +635,7 @@ Launch plan_launch(const std::vector<KvSeq>& seqs, const KvView& kv, const Paged
     groups *= kv.kv_heads;
     // pages of a part: as many workgroups as the card takes at a time, unless
     // the tiles alone are
-    const int least = many ? 1 : 4 * kFewWaves;
+    const int least = many ? 8 : 4 * kFewWaves;
     const int target = many ? kTargetMany : kTarget;
     long long chunk = std::max<long long>(least, (work + target - 1) / target);
     if (many && groups >= target / 2) chunk = 2ll * longest;
@@ -650,13 +655,14 @@ template <int HD, int R, int NW, bool PAGES>
 int launch_one(hipStream_t s, const Launch& l, const KvView& kv, const KvPlanView& p, const PagedArgs& a) {
     const float scale = 1.4426950408889634f / sqrtf((float)HD);  // scores in units of log 2
     const size_t grid = (size_t)l.cut.tiles * kv.kv_heads;
-    const size_t merge = (size_t)l.cut.rows_hi * kv.kv_heads;
+    constexpr int W = PAGES ? 4 : 1;  // wavefronts that share a row of the merge
+    const size_t merge = (size_t)(l.cut.rows_hi * W + 3) / 4 * kv.kv_heads;
     if (grid > (size_t)INT32_MAX || merge > (size_t)INT32_MAX)
         return set_error(SQ_ERR_SHAPE, "sdpa_paged: ShapeMismatch (too many rows)");
     hipLaunchKernelGGL((sdpa_paged_kernel<HD, R, NW, PAGES>), dim3((unsigned)grid, l.cut.splits, p.n_seqs), dim3(NW * 64), 0, s, kv, p, a,
                        l.cut, scale);
     if (l.cut.splits > 1)
-        hipLaunchKernelGGL((sdpa_merge_kernel<HD>), dim3((unsigned)merge, p.n_seqs), dim3(256), 0, s, kv, p, a, l.cut,
+        hipLaunchKernelGGL((sdpa_merge_kernel<HD, W>), dim3((unsigned)merge, p.n_seqs), dim3(256), 0, s, kv, p, a, l.cut,
                            PAGES ? 16 * R : NW * 16 * R);
     return check_launch("sdpa_paged");
 }

@@ -303,17 +303,17 @@ def sdpa_paged(plan: KvPlan, layer: int, q: DeviceArray, out: DeviceArray, n_hea
 def verify_draft(target: DeviceArray, draft: DeviceArray | None, tokens: DeviceArray, u: DeviceArray, n_draft,
                  temperature: float) -> tuple[np.ndarray, np.ndarray]:
     """Accepted drafts and the next token of each sequence (sq_verify_draft)."""
-    n = np.asarray(n_draft)
-    if n.ndim != 1 or (n.size and (n.min() < 0 or n.max() > 0xFFFFFFFF)):
+    n = np.ascontiguousarray(n_draft).astype(np.uint32, copy=False)  # (a negative count is more than 1024: refused)
+    if n.ndim != 1:
         _shape_error()
-    n = np.ascontiguousarray(n, dtype=np.uint32)
-    drafts = int(n.astype(np.int64).sum())
-    if len(target.shape) != 2 or target.shape[0] != drafts + n.size or tokens.size != drafts or u.size != drafts + n.size:
+    seqs, drafts = n.size, int(n.sum(dtype=np.int64))
+    if len(target.shape) != 2 or target.shape[0] != drafts + seqs or tokens.size != drafts or u.size != drafts + seqs:
         _shape_error()
     vocab = target.shape[1]
     if draft is not None and draft.shape != (drafts, vocab):
         _shape_error()
-    accepted, token = np.zeros(n.size, np.uint32), np.zeros(n.size, np.uint32)
+    out = np.empty((2, seqs), np.uint32)
+    at = out.__array_interface__["data"][0]
     check(lib().sq_verify_draft(target.ptr, vocab, draft.ptr if draft is not None else None, vocab, tokens.ptr, u.ptr,
-                                n.ctypes.data, n.size, vocab, temperature, accepted.ctypes.data, token.ctypes.data))
-    return accepted, token
+                                n.__array_interface__["data"][0], seqs, vocab, temperature, at, at + 4 * seqs))
+    return out[0], out[1]

@@ -18,7 +18,8 @@ def emulated():
 
 
 @pytest.mark.parametrize("tests", ["refusals or nothing", "append or growing or partial or far or zero_and or apart",
-                                   "layers or finite or flat or rotated or bad_queries or batch", "test_sdpa_paged",
+                                   "layers or finite or flat or rotated or bad_queries or batch or very_different",
+                                   "test_sdpa_paged",
                                    "verify or rejection", "serving_steps"])
 @pytest.mark.parametrize("reverse", ["0", "1"])
 def test_small_cases_on_the_emulator(emulated, tests, reverse):

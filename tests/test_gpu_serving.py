@@ -246,6 +246,11 @@ SDPA = [
     ("small", 64, 2, 2, [(0, 140)], 5, 70),
     ("small", 64, 2, 1, [(200, 3)], 1 << 31, 1 << 31),
     ("small", 128, 8, 1, [(500, 2), (3, 1)], 130, 1),
+    # pages in parts, of few rows and of many
+    ("small", 64, 4, 2, [(1600, 2), (5, 1)], 0, 0),
+    ("small", 64, 1, 1, [(760, 66)], 0, 0),
+    ("small", 128, 2, 1, [(700, 40), (20, 33), (3, 1)], 0, 0),
+    ("small", 64, 2, 1, [(1700, 3), (900, 50)], 800, 70),
     ("large", 64, 32, 8, [(300, 1)], 0, 0),
     ("large", 64, 32, 8, [(0, 1), (5000, 1), (64, 1), (1023, 1), (77, 1), (2048, 1)], 0, 0),
     ("large", 64, 32, 8, [(2000, 5), (100, 3), (0, 6), (700, 1)], 0, 0),
@@ -269,6 +274,23 @@ def test_sdpa_paged(size, dim, heads, kv_heads, seqs, window, sinks):
     t.append([0] * len(seqs), past)
     plan = t.append(past, new)
     t.attend(plan, past, new, heads, window, sinks)
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_sdpa_pages_of_very_different_size_small(rows):
+    """Values (and keys) whose magnitude changes by page, up and down by up to
+    2^100, with pages of zeros between: the sums' unit follows them."""
+    n = 64 * 9
+    t = Step([n + rows], 1, 64, half=0, seed=18 + rows)
+    k, v = t.rows(n)
+    size = np.array([1, 2.0**9, 2.0**-9, 0, 2.0**60, 2.0**-40, 2.0**-7, 2.0**7, 1], np.float32)
+    v = v * np.repeat(size, 64)[:, None]
+    k = k * np.repeat(np.array([1, 3, 1e-6, 1, 0, 1, 2, 1, 1], np.float32), 64)[:, None]
+    for chosen in (size > 0, size < 2.0**50):  # the second: without the huge page
+        keep = np.repeat(chosen, 64)
+        t.append([0], [n], rows=(k, np.where(keep[:, None], v, 0)))
+        plan = t.append([n], [rows])
+        t.attend(plan, [n], [rows], 2)
 
 
 @pytest.mark.parametrize("scale", [1e-3, 8.0])
@@ -337,6 +359,25 @@ def test_sdpa_repeats_bit_for_bit():
         ops.sdpa_paged(plan, 0, q, out, 32)
         outs.append(out.numpy())
     assert all(np.array_equal(o, outs[0]) for o in outs)
+
+
+def test_many_sequences_and_long_mixed_batch():
+    """A decode batch of 700 sequences, and one with a long chat, a prompt and
+    single tokens together (both kernels, cut and uncut pages)."""
+    r = rng(30)
+    past = list(r.integers(0, 130, 700))
+    new = list(r.integers(0, 3, 700))
+    t = Step([int(a + b) for a, b in zip(past, new)], 2, 64, seed=31)
+    t.append([0] * 700, past)
+    plan = t.append(past, new)
+    t.check_cache(plan, past, new)
+    t.attend(plan, past, new, 4)
+    past, new = [20000, 40, 0, 700, 64], [1, 200, 1, 3, 64]
+    t = Step([a + b for a, b in zip(past, new)], 2, 64, seed=32)
+    t.append([0] * 5, past)
+    plan = t.append(past, new)
+    t.attend(plan, past, new, 8)
+    t.attend(plan, past, new, 8, 1000, 5)
 
 
 def test_pages_past_4_gib():
