@@ -607,10 +607,7 @@ int sq_sdpa_paged(sq_kv_plan* plan, size_t layer, const float* d_q, size_t q_str
     const PagedArgs a{d_q,        q_stride,     d_out,
                       out_stride, (int)n_heads, window < longest ? (int)window : 0,
                       (int)std::min(n_sinks, longest)};
-    Tmp ws;
-    const size_t floats = sdpa_paged_floats(plan->seqs, kv, a);
-    if (floats && (st = ws.alloc(floats * sizeof(float)))) return finish(st);
-    return finish(launch_sdpa_paged(nullptr, plan->seqs, kv, pv, a, (float*)ws.p));
+    return finish(launch_sdpa_paged(plan->seqs, kv, pv, a));
 }
 
 int sq_verify_draft(const float* d_target, size_t target_stride, const float* d_draft, size_t draft_stride,
@@ -645,7 +642,8 @@ int sq_verify_draft(const float* d_target, size_t target_stride, const float* d_
         VerifyBatch b;
         memset(&b, 0, sizeof(b));
         size_t rows = 0;
-        while (b.n_seqs < (uint32_t)kVerifySeqs && s0 + b.n_seqs < n_seqs) {
+        while (b.n_seqs < (uint32_t)kVerifySeqs && s0 + b.n_seqs < n_seqs &&
+               (b.n_seqs == 0 || verify_fits(2 * (rows + n_draft[s0 + b.n_seqs] + 1), (int)vocab))) {
             b.target0[b.n_seqs] = (uint32_t)rows;
             b.n[b.n_seqs] = (uint16_t)n_draft[s0 + b.n_seqs];
             rows += n_draft[s0 + b.n_seqs] + 1;

@@ -231,7 +231,7 @@ int launch_kv_rope(hipStream_t s, const KvPlanView& p, const float* inv_freq, in
 int launch_kv_append(hipStream_t s, const KvView& kv, const KvPlanView& p, const float* k, size_t k_stride,
                      const float* v, size_t v_stride, uint32_t* bad) {
     const size_t grid = (size_t)p.n_items * kv.kv_heads;
-    if (grid > (size_t)INT32_MAX) return set_error(SQ_ERR_SHAPE, "kv_append: ShapeMismatch (too many pages)");
+    if (!grid_fits(grid, 4 * kv.head_dim)) return set_error(SQ_ERR_SHAPE, "kv_append: ShapeMismatch (too many pages)");
     if (kv.head_dim == 64)
         hipLaunchKernelGGL(kv_append_kernel<64>, dim3((unsigned)grid, 2), dim3(256), 0, s, kv, p.items, p.rope,
                            p.half, k, k_stride, v, v_stride, bad);
@@ -244,7 +244,7 @@ int launch_kv_append(hipStream_t s, const KvView& kv, const KvPlanView& p, const
 int launch_kv_read(hipStream_t s, const KvView& kv, const KvPlanView& p, int last, int max_pages, float* k_out,
                    float* v_out) {
     const size_t grid = (size_t)max_pages * kv.kv_heads;
-    if (grid > (size_t)INT32_MAX) return set_error(SQ_ERR_SHAPE, "kv_read: ShapeMismatch (too many pages)");
+    if (!grid_fits(grid, 4 * kv.head_dim)) return set_error(SQ_ERR_SHAPE, "kv_read: ShapeMismatch (too many pages)");
     if (kv.head_dim == 64)
         hipLaunchKernelGGL(kv_read_kernel<64>, dim3((unsigned)grid, p.n_seqs, 2), dim3(256), 0, s, kv, p, last, k_out, v_out);
     else

@@ -8,6 +8,7 @@
 #include <cmath>
 
 #include "kv.h"
+#include "scratch.h"
 
 namespace sq {
 namespace {
@@ -598,10 +599,20 @@ __global__ __launch_bounds__(256) void sdpa_merge_kernel(KvView kv, KvPlanView p
     for (int c = 0; c < C; c++) out[64 * c + lane] = o[c] * (unit / ll);
 }
 
-// Sequences of few rows: wavefronts over pages, tiles of 16 rows; of more: wavefronts over
-// rows, tiles of 128 (of 64 with 128 dimensions, whose sums take the registers of two).
-constexpr int kFewWaves = 4, kFewRows = 64, kTileFew = 16, kTileMany = 64;
-constexpr int kTarget = 768, kTargetMany = 512;  // workgroups that a launch is cut into
+// Sequences of few rows: wavefronts over pages, tiles of 16 rows, which read
+// the pages once each (from the L2 after the first).  More rows: wavefronts over
+// rows, tiles of 64, a page unpacked once for all of them.  Measured on 32
+// sequences of 8 KV heads, 64 dimensions, 512 / 4096 positions (us): 40 rows 11 /
+// 47 by pages and 15 / 86 by rows, 96 rows 19 / 83 and 19 / 104, 128 rows 23 /
+// 107 and 19 / 102; with 128 dimensions 96 rows 33 / 158 and 29 / 166.
+constexpr int kFewWaves = 4, kFewRows = 96, kTileFew = 16, kTileMany = 64;
+// Pages are cut into parts until the launch has about so many workgroups (three
+// a CU by pages; fewer and 48 chats of up to 8000 positions take 25 us instead
+// of 22), of at least 16 pages by pages (four a wavefront) and 8 by rows.  Tiles
+// of rows that are half as many as the target already are not cut: the merge's
+// traffic costs more than the idle CUs (1024 rows behind 8192: 205 us uncut,
+// 185 + 19 in two parts).
+constexpr int kTarget = 768, kTargetMany = 512;
 
 struct Launch {
     Cut cut;
@@ -633,8 +644,6 @@ Launch plan_launch(const std::vector<KvSeq>& seqs, const KvView& kv, const Paged
     }
     work *= kv.kv_heads;
     groups *= kv.kv_heads;
-    // pages of a part: as many workgroups as the card takes at a time, unless
-    // the tiles alone are
     const int least = many ? 8 : 4 * kFewWaves;
     const int target = many ? kTargetMany : kTarget;
     long long chunk = std::max<long long>(least, (work + target - 1) / target);
@@ -652,41 +661,38 @@ Launch plan_launch(const std::vector<KvSeq>& seqs, const KvView& kv, const Paged
 }
 
 template <int HD, int R, int NW, bool PAGES>
-int launch_one(hipStream_t s, const Launch& l, const KvView& kv, const KvPlanView& p, const PagedArgs& a) {
+int launch_one(const Launch& l, const KvView& kv, const KvPlanView& p, const PagedArgs& a) {
     const float scale = 1.4426950408889634f / sqrtf((float)HD);  // scores in units of log 2
     const size_t grid = (size_t)l.cut.tiles * kv.kv_heads;
     constexpr int W = PAGES ? 4 : 1;  // wavefronts that share a row of the merge
     const size_t merge = (size_t)(l.cut.rows_hi * W + 3) / 4 * kv.kv_heads;
-    if (grid > (size_t)INT32_MAX || merge > (size_t)INT32_MAX)
+    if (!grid_fits(grid, NW * 64) || !grid_fits(merge, 256))
         return set_error(SQ_ERR_SHAPE, "sdpa_paged: ShapeMismatch (too many rows)");
-    hipLaunchKernelGGL((sdpa_paged_kernel<HD, R, NW, PAGES>), dim3((unsigned)grid, l.cut.splits, p.n_seqs), dim3(NW * 64), 0, s, kv, p, a,
-                       l.cut, scale);
+    hipLaunchKernelGGL((sdpa_paged_kernel<HD, R, NW, PAGES>), dim3((unsigned)grid, l.cut.splits, p.n_seqs),
+                       dim3(NW * 64), 0, nullptr, kv, p, a, l.cut, scale);
     if (l.cut.splits > 1)
-        hipLaunchKernelGGL((sdpa_merge_kernel<HD, W>), dim3((unsigned)merge, p.n_seqs), dim3(256), 0, s, kv, p, a, l.cut,
+        hipLaunchKernelGGL((sdpa_merge_kernel<HD, W>), dim3((unsigned)merge, p.n_seqs), dim3(256), 0, nullptr, kv, p, a, l.cut,
                            PAGES ? 16 * R : NW * 16 * R);
     return check_launch("sdpa_paged");
 }
 
 }  // namespace
 
-size_t sdpa_paged_floats(const std::vector<KvSeq>& seqs, const KvView& kv, const PagedArgs& a) {
-    return std::max(plan_launch(seqs, kv, a, false).floats, plan_launch(seqs, kv, a, true).floats);
-}
-
-int launch_sdpa_paged(hipStream_t s, const std::vector<KvSeq>& seqs, const KvView& kv, const KvPlanView& p,
-                      const PagedArgs& a, float* ws) {
-    for (bool many : {false, true}) {
-        Launch l = plan_launch(seqs, kv, a, many);
-        if (!l.any) continue;
-        l.cut.ws = ws;
-        int st;
+int launch_sdpa_paged(const std::vector<KvSeq>& seqs, const KvView& kv, const KvPlanView& p, const PagedArgs& a) {
+    Launch l[2] = {plan_launch(seqs, kv, a, false), plan_launch(seqs, kv, a, true)};
+    Tmp ws;  // (the second launch follows the first's merge)
+    const size_t floats = std::max(l[0].floats, l[1].floats);
+    int st = 0;
+    if (floats && (st = ws.alloc(floats * sizeof(float)))) return st;
+    for (int many = 0; many < 2 && !st; many++) {
+        if (!l[many].any) continue;
+        l[many].cut.ws = (float*)ws.p;
         if (kv.head_dim == 64)
-            st = many ? launch_one<64, 1, 4, false>(s, l, kv, p, a) : launch_one<64, 1, kFewWaves, true>(s, l, kv, p, a);
+            st = many ? launch_one<64, 1, 4, false>(l[1], kv, p, a) : launch_one<64, 1, kFewWaves, true>(l[0], kv, p, a);
         else
-            st = many ? launch_one<128, 1, 4, false>(s, l, kv, p, a) : launch_one<128, 1, kFewWaves, true>(s, l, kv, p, a);
-        if (st) return st;
+            st = many ? launch_one<128, 1, 4, false>(l[1], kv, p, a) : launch_one<128, 1, kFewWaves, true>(l[0], kv, p, a);
     }
-    return 0;
+    return st;
 }
 
 }  // namespace sq

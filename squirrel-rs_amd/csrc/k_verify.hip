@@ -400,6 +400,8 @@ size_t align16(size_t n) { return (n + 15) & ~(size_t)15; }
 
 }  // namespace
 
+bool verify_fits(size_t rows, int vocab) { return grid_fits(rows * (((size_t)vocab + kChunk - 1) / kChunk), kPartBlock); }
+
 size_t verify_ws_bytes(size_t rows, size_t n_seqs, int vocab) {
     const size_t chunks = ((size_t)vocab + kChunk - 1) / kChunk;
     return align16(rows * chunks * sizeof(Part)) + align16(n_seqs * chunks * sizeof(double)) + n_seqs * sizeof(Choice);
@@ -412,7 +414,7 @@ int launch_verify(hipStream_t s, const VerifyBatch& b, const VerifyArgs& a, size
     Part* parts = (Part*)ws;
     double* sums = (double*)((char*)ws + align16(rows * chunks * sizeof(Part)));
     Choice* choices = (Choice*)((char*)sums + align16((size_t)b.n_seqs * chunks * sizeof(double)));
-    if (rows * chunks > (size_t)INT32_MAX) return set_error(SQ_ERR_SHAPE, "verify_draft: ShapeMismatch (too many logits)");
+    if (!verify_fits(rows, a.vocab)) return set_error(SQ_ERR_SHAPE, "verify_draft: ShapeMismatch (too many logits)");
     auto kernel = a.inv_t == 0.0 ? verify_parts_kernel<true> : verify_parts_kernel<false>;
     hipLaunchKernelGGL(kernel, dim3((unsigned)(rows * chunks)), dim3(kPartBlock), 0, s, a, (int)target_rows, chunks, parts);
     hipLaunchKernelGGL(verify_sums_kernel, dim3(std::min(chunks, std::max(1, kSumGroups / (int)b.n_seqs)), b.n_seqs),

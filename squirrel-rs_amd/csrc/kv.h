@@ -82,10 +82,8 @@ struct PagedArgs {
     size_t out_stride;
     int heads, window, sinks;
 };
-// Floats of workspace that launch_sdpa_paged needs for these sequences.
-size_t sdpa_paged_floats(const std::vector<KvSeq>& seqs, const KvView& kv, const PagedArgs& a);
-int launch_sdpa_paged(hipStream_t s, const std::vector<KvSeq>& seqs, const KvView& kv, const KvPlanView& p,
-                      const PagedArgs& a, float* ws);
+// (on the null stream, with a workspace from the scratch pool)
+int launch_sdpa_paged(const std::vector<KvSeq>& seqs, const KvView& kv, const KvPlanView& p, const PagedArgs& a);
 
 }  // namespace sq
 

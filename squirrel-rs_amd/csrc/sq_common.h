@@ -97,6 +97,10 @@ __host__ __device__ inline size_t frag_scale(int rows, int kblocks, int row, int
     return base + ((size_t)(kb >> 1) * rt + r) * 2 + (kb & 1);
 }
 
+// Whether a launch of `groups` workgroups along one axis is within the runtime's
+// limit of 2^32 - 1 work-items.
+inline bool grid_fits(size_t groups, size_t threads) { return groups <= (size_t)UINT32_MAX / threads; }
+
 inline MatView view(const DevMatrix& m) { return MatView{m.qs, m.scale, m.rows, m.k, m.wtype}; }
 
 }  // namespace sq

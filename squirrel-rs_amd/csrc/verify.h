@@ -29,6 +29,8 @@ struct VerifyResult {
     uint32_t accepted, token, bad, pad;
 };
 
+// Whether one launch takes so many target and draft rows.
+bool verify_fits(size_t rows, int vocab);
 // Bytes of workspace for `rows` target and draft rows and n_seqs sequences.
 size_t verify_ws_bytes(size_t rows, size_t n_seqs, int vocab);
 int launch_verify(hipStream_t s, const VerifyBatch& b, const VerifyArgs& a, size_t target_rows, size_t draft_rows,

@@ -251,6 +251,9 @@ SDPA = [
     ("small", 64, 1, 1, [(760, 66)], 0, 0),
     ("small", 128, 2, 1, [(700, 40), (20, 33), (3, 1)], 0, 0),
     ("small", 64, 2, 1, [(1700, 3), (900, 50)], 800, 70),
+    ("small", 64, 1, 1, [(860, 97)], 0, 0),
+    ("small", 128, 3, 1, [(700, 40), (20, 33), (3, 1)], 0, 0),
+    ("small", 64, 4, 1, [(1100, 30), (40, 25)], 900, 70),
     ("large", 64, 32, 8, [(300, 1)], 0, 0),
     ("large", 64, 32, 8, [(0, 1), (5000, 1), (64, 1), (1023, 1), (77, 1), (2048, 1)], 0, 0),
     ("large", 64, 32, 8, [(2000, 5), (100, 3), (0, 6), (700, 1)], 0, 0),
@@ -276,7 +279,7 @@ def test_sdpa_paged(size, dim, heads, kv_heads, seqs, window, sinks):
     t.attend(plan, past, new, heads, window, sinks)
 
 
-@pytest.mark.parametrize("rows", [1, 40])
+@pytest.mark.parametrize("rows", [1, 40, 60])
 def test_sdpa_pages_of_very_different_size_small(rows):
     """Values (and keys) whose magnitude changes by page, up and down by up to
     2^100, with pages of zeros between: the sums' unit follows them."""
