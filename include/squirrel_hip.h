@@ -273,9 +273,10 @@ int sq_log_softmax_at(const float* d_logits, size_t n, uint32_t idx, double* out
  *
  * One step: describe it once in a plan, then for every layer append the new
  * keys and values and attend.  Calls run on the null stream and return
- * finished.  A plan belongs to one thread at a time; a pool may be shared by
- * plans whose steps write different pages.  Free plans before their pool.  Every call needs the
- * pool's device to be the current one (SQ_ERR_ARG otherwise). */
+ * finished, so they cannot be recorded under a stream capture.  A plan belongs to
+ * one thread at a time; a pool may be shared by plans whose steps write
+ * different pages.  Free plans before their pool.  Every call needs the pool's
+ * device to be the current one (SQ_ERR_ARG otherwise). */
 #define SQ_KV_PAGE 64
 #define SQ_KV_ROTATED 1u /* the rows are rotated already */
 typedef struct sq_kv_pool sq_kv_pool;
@@ -303,11 +304,12 @@ int sq_kv_plan_set(sq_kv_plan* plan, size_t n_seqs, const uint32_t* past, const 
 void sq_kv_plan_free(sq_kv_plan* plan);
 /* Rotates the batch's keys (not with SQ_KV_ROTATED), quantizes keys and
  * values and writes them.  Strides in floats, at least kv_heads * head_dim.
- * The scale of a page whose first row is new is f32(max|x| / 127) over its new rows;
- * behind earlier rows it is that or the page's former scale, whichever is larger, and
- * where it grows the earlier rows' integers become rint(q * s_old / s).  A
- * value x is stored as rint(x / s).  A row that is not finite is SQ_ERR_ARG: it is
- * stored as zero (a key's whole pair), everything else of the call as it should be. */
+ * The scale of a page whose first row is new is f32(max|x| / 127) over its new
+ * rows; behind earlier rows it is that or the page's former scale, whichever is
+ * larger, and where it grows the earlier rows' integers become
+ * rint(q * s_old / s).  A value x is stored as rint(x / s), all of it decided in
+ * 64 bits.  A value that is not finite is SQ_ERR_ARG: it is stored as zero (a
+ * key's whole pair), everything else of the call as it should be. */
 int sq_kv_append(sq_kv_plan* plan, size_t layer, const float* d_k, size_t k_stride,
                  const float* d_v, size_t v_stride, uint32_t flags);
 /* The cached values of the last min(last, past + n_new) positions of every
@@ -318,7 +320,10 @@ int sq_kv_read(sq_kv_plan* plan, size_t layer, size_t last, float* d_k, float* d
  * (rotated on the way, not with SQ_KV_ROTATED) and d_out hold n_heads *
  * head_dim floats a row, strides in floats.  A query at position p sees the
  * positions j <= p, with a window (> 0) those with j > p - window or j <
- * n_sinks.  f32 results as sq_sdpa's over the cached values.  d_out may be d_q. */
+ * n_sinks.  f32 results as sq_sdpa's over the cached values (within 2^96 of the
+ * sequence's first page: the value scales of further pages count as no more than that
+ * larger or smaller).  A query row that is not finite gives NaN in its own head's
+ * row and nowhere else.  d_out may be d_q with the same stride. */
 int sq_sdpa_paged(sq_kv_plan* plan, size_t layer, const float* d_q, size_t q_stride, float* d_out,
                   size_t out_stride, size_t n_heads, size_t window, size_t n_sinks,
                   uint32_t flags);
@@ -334,7 +339,9 @@ int sq_sdpa_paged(sq_kv_plan* plan, size_t layer, const float* d_q, size_t q_str
  * Temperature 0: accepted while a draft is sq_greedy's token, next is sq_greedy's.
  * In 64 bits throughout.  Logits may be -inf (probability 0); a row on which the
  * result depends that holds NaN or +inf or nothing above -inf, or an id past the
- * vocabulary, is SQ_ERR_ARG, and the results are left as they were. */
+ * vocabulary, is SQ_ERR_ARG, and the results are left as they were.  (Where the
+ * weights of a rejected draft are zero throughout, p and q agree everywhere: the
+ * token is drawn from p.) */
 int sq_verify_draft(const float* d_target, size_t target_stride, const float* d_draft,
                     size_t draft_stride, const uint32_t* d_tokens, const float* d_u,
                     const uint32_t* n_draft, size_t n_seqs, size_t vocab, float temperature,

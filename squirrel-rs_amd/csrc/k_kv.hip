@@ -66,9 +66,9 @@ constexpr int kFewTokens = 16;
 //   bytes of keys a lane, or two single ones of values);
 //   otherwise through an image of the page in LDS, written out 16 bytes a
 //   thread; earlier rows of the page are in it, in the steps of the new scale.
-// Bound by latency for single tokens, by the reads and about 20 f64 operations
-// a value for whole pages.  (Keys and values in one workgroup: 10.7 us for 2011
-// rows of 8 x 128, one page of a head a CU with nothing to overlap.)
+// Bound by latency for single tokens (one: 3.4 us, 96 sequences with one each:
+// 5.6), by the chain read - maximum - quantize - write for whole pages: 2011 rows
+// of 8 x 128 are 20.6 MB in 10.2 us, two workgroups a CU.
 template <int HD, bool VALUES>
 __device__ __forceinline__ void append_page(const KvView& kv, const KvItem& it, int head,
                                             const double2* __restrict__ rope, int half, const float* __restrict__ in,
@@ -173,7 +173,7 @@ __global__ __launch_bounds__(HD * 4) void kv_append_kernel(KvView kv, const KvIt
 
 // One workgroup per (sequence, page of its last positions, KV head) and one of
 // keys and values: the page's bytes through LDS, four dimensions a thread on the
-// way out.
+// way out.  Bound by the writes: 2048 rows of 8 x 128 (21 MB) in 8.6 us.
 template <int HD>
 __global__ __launch_bounds__(HD * 4) void kv_read_kernel(KvView kv, KvPlanView p, int last, float* __restrict__ k_out,
                                                          float* __restrict__ v_out) {
@@ -245,10 +245,9 @@ int launch_kv_read(hipStream_t s, const KvView& kv, const KvPlanView& p, int las
                    float* v_out) {
     const size_t grid = (size_t)max_pages * kv.kv_heads;
     if (!grid_fits(grid, 4 * kv.head_dim)) return set_error(SQ_ERR_SHAPE, "kv_read: ShapeMismatch (too many pages)");
-    if (kv.head_dim == 64)
-        hipLaunchKernelGGL(kv_read_kernel<64>, dim3((unsigned)grid, p.n_seqs, 2), dim3(256), 0, s, kv, p, last, k_out, v_out);
-    else
-        hipLaunchKernelGGL(kv_read_kernel<128>, dim3((unsigned)grid, p.n_seqs, 2), dim3(512), 0, s, kv, p, last, k_out, v_out);
+    auto kernel = kv.head_dim == 64 ? kv_read_kernel<64> : kv_read_kernel<128>;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)grid, p.n_seqs, 2), dim3(4 * kv.head_dim), 0, s, kv, p, last, k_out,
+                       v_out);
     return check_launch("kv_read");
 }
 

@@ -25,8 +25,9 @@ inline int check_launch(const char* what) {
 }
 
 // Division of x < 2^31 by a number that a launch knows: with m = ceil(2^32 / d)
-// floor(x m / 2^32) is the quotient or one more.  (The dozen divisions at a workgroup's
-// start cost 1.5 us of one token's 5.5 as the compiler makes them.)
+// floor(x m / 2^32) is the quotient or one more.  (With the dozen divisions of a
+// workgroup's start as the compiler makes them a token over 300 positions took
+// 7.3 us instead of 5.7.)
 struct alignas(8) Div {
     uint32_t d, m;  // (m = 0: d = 1)
     Div() = default;
@@ -61,8 +62,9 @@ __host__ __device__ inline Span tile_span(int pos_lo, int pos_hi, int window, in
 
 // What a launch covers: the sequences with rows_lo <= n_new * G <= rows_hi,
 // their pages cut into parts of `chunk` (the last one holds between a half and
-// one and a half of it).  The parts' sums stand in the workspace at slot (table0 / chunk + sequence + part): a sequence has
-// at most pages / chunk + 1 parts, so slots do not overlap.
+// one and a half of it).  The parts' sums stand in the workspace at slot
+// (table0 / chunk + sequence + part): a sequence has at most pages / chunk + 1
+// parts, so slots do not overlap.
 struct Cut {
     int rows_lo, rows_hi, chunk, tiles, splits, pad;
     Div by_chunk, by_group, by_heads;  // chunk, heads / kv_heads, kv_heads
@@ -100,7 +102,9 @@ __device__ __forceinline__ float groups_sum(float v) {
 // Scales of a sequence's pages are taken relative to its first page's (1 where
 // that holds zeros), within 2^96 of it either way: their quotients stay in f32.
 // A page of zeros may have any scale.
-__device__ __forceinline__ float first_unit(float scale) { return scale > 0.0f ? fminf(fmaxf(scale, 0x1p-30f), 0x1p30f) : 1.0f; }
+__device__ __forceinline__ float first_unit(float scale) {
+    return scale > 0.0f ? fminf(fmaxf(scale, 0x1p-30f), 0x1p30f) : 1.0f;
+}
 __device__ __forceinline__ float page_unit(float scale, float unit) {
     return scale > 0.0f ? fminf(fmaxf(scale, unit * 0x1p-96f), unit * 0x1p96f) : unit;
 }
@@ -173,38 +177,49 @@ __device__ __forceinline__ void halves(float x, int shift, _Float16& h, _Float16
 // stay within kHeadroom of it nothing is rescaled, and the operands stay below
 // 2^(kBase + kHeadroom), in f16's range with kBase bits of room for small ones.
 //
-// PAGES: the wavefronts take pages in turn for the same 16 R rows and meet in
-// LDS; otherwise each has its own 16 R rows and all walk the same pages.
+// PAGES: the wavefronts take pages in turn for the same 16 rows and meet in LDS;
+// otherwise each has its own 16 rows and all walk the same pages.  (32 rows a
+// wavefront leave two of them a SIMD: 73 us instead of 55 for 1531 rows.)
+//
+// What bounds them.  By pages: the reads of the cache, from about 32 pages a
+// sequence on (256 sequences and heads of 4096 positions: 134 MB in 24 us, 5.6
+// TB/s; 131000 positions of one: 25 us); below that the chain from the launch's
+// arguments to a page's bytes and the meeting in LDS, 6 us (300 positions).  By
+// rows: the VALU's softmax and halves beside the matrix pipe, 443 TFLOP/s for
+// 8192 rows of 32 heads of 64 (two f16 products for one of f32: 577 at the rate
+// of a large f16 product), and about 12 us of start and end: 50 us for 1531
+// rows behind 517.
 constexpr int kStat = 4;  // floats behind a part's sums: the maximum, the sum of weights, two unused
 constexpr float kBase = 8.0f, kHeadroom = 6.0f;
-template <int HD, int R, int NW, bool PAGES>
-__global__ __launch_bounds__(NW * 64, PAGES ? (HD == 64 ? 3 : 2) : (HD == 64 ? 4 : 2)) void sdpa_paged_kernel(KvView kv, KvPlanView pl, PagedArgs a, Cut cut, float scale) {
-    constexpr int C = HD / 64, DT = HD / 16, TR = PAGES ? 16 * R : NW * 16 * R;
-    __shared__ __attribute__((aligned(16))) float s_o[PAGES ? NW * 16 * R * (HD + 4) : 1];
-    __shared__ __attribute__((aligned(16))) _Float16 s_q[2][PAGES ? 16 * R * HD : 8];
-    __shared__ float s_cq[PAGES ? 16 * R : 1];
+template <int HD, int NW, bool PAGES>
+__global__ __launch_bounds__(NW * 64, HD != 64 ? 2 : PAGES ? 3 : 4) void sdpa_paged_kernel(KvView kv, KvPlanView pl,
+                                                                                          PagedArgs a, Cut cut,
+                                                                                          float scale) {
+    constexpr int C = HD / 64, DT = HD / 16, TR = PAGES ? 16 : NW * 16;
+    __shared__ __attribute__((aligned(16))) float s_o[PAGES ? NW * 16 * (HD + 4) : 1];
+    __shared__ __attribute__((aligned(16))) _Float16 s_q[2][PAGES ? 16 * HD : 8];
+    __shared__ float s_cq[PAGES ? 16 : 1];
     __shared__ __attribute__((aligned(16))) v8h s_kv[PAGES ? 1 : 2][PAGES ? 1 : 16 * C * 64];
-    __shared__ float s_m[PAGES ? NW * 16 * R : 1], s_l[PAGES ? NW * 16 * R : 1];
+    __shared__ float s_m[PAGES ? NW * 16 : 1], s_l[PAGES ? NW * 16 : 1];
     // (heads next to each other: with eight of them each is one XCD's, and a
-    // head's tiles share that XCD's L2.  A sequence's last tiles see the most pages:
-    // they come first, and every second 32 of a head's, one for each CU of an XCD,
-    // in the other order, so that the CUs' shares are alike)
-    const int at = cut.by_heads(blockIdx.x), head = blockIdx.x - at * kv.kv_heads;
-    const int from = at & ~31, turned = (at & 32) ? from + min(cut.tiles, from + 32) - 1 - at : at;
-    const int tile = cut.tiles - 1 - turned;
+    // head's tiles share that XCD's L2.  A sequence's last tiles, which see the most
+    // pages, come first)
+    const int at = cut.by_heads(blockIdx.x), head = blockIdx.x - at * kv.kv_heads, tile = cut.tiles - 1 - at;
     const int part = blockIdx.y, seq = blockIdx.z;
     const KvSeq s = pl.seqs[seq];
     const int G = (int)cut.by_group.d, rows = s.n_new * G;
     if (rows < cut.rows_lo || rows > cut.rows_hi || tile * TR >= rows) return;
     const int row_end = min(rows, (tile + 1) * TR);
-    const Span span = tile_span(s.past + cut.by_group(tile * TR), s.past + cut.by_group(row_end - 1), a.window, a.sinks);
+    const Span span =
+        tile_span(s.past + cut.by_group(tile * TR), s.past + cut.by_group(row_end - 1), a.window, a.sinks);
     const int parts = cut.parts(span.count);
     if (part >= parts) return;
     const int i_end = part == parts - 1 ? span.count : (part + 1) * cut.chunk;
     const bool whole = parts == 1;
 
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, q16 = lane & 15, g = lane >> 4;
-    const int row0 = tile * TR + (PAGES ? 0 : wave * 16 * R);  // the wavefront's first row
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, q16 = lane & 15, g = lane >> 4;
+    const int row0 = tile * TR + (PAGES ? 0 : wave * 16);  // the wavefront's first row
 
     // A page's bytes are 8 C pieces of 1 KB, one load of a wavefront each: keys,
     // then values.
@@ -212,8 +227,8 @@ __global__ __launch_bounds__(NW * 64, PAGES ? (HD == 64 ? 3 : 2) : (HD == 64 ? 4
     // before the second product, its values behind it.
     // Otherwise the wavefronts share the work on a page: each loads and unpacks
     // its pieces of the page after next into one of two f16 images in LDS.
-    // (Unpacked by every wavefront for itself that was 128 of 286 VALU
-    // instructions for 16 rows of a page: 62 us against 4x for a prompt's 1531 rows.)
+    // (Unpacked by every wavefront for itself that is 128 of 286 VALU
+    // instructions for 16 rows of a page: 62 us instead of 55 for 1531 rows.)
     constexpr int P = 8 * C, OWN = PAGES ? P : P / NW;
     static_assert(PAGES || P % NW == 0, "whole pieces a wavefront");
     const int step = PAGES ? NW : 1;
@@ -250,30 +265,25 @@ __global__ __launch_bounds__(NW * 64, PAGES ? (HD == 64 ? 3 : 2) : (HD == 64 ? 4
     const float unit = first_unit(kv.scales[(size_t)pl.pages[s.table0] * kv.kv_heads + head].y);
 
     // Queries: [chunk of 64][half of a lane's 16 dimensions].
-    v8h qh[R][C][2], ql[R][C][2];
-    float cq[R];
-    int pos[R], w0[R];
+    v8h qh[C][2], ql[C][2];
+    float cq;
     const bool vec = (((uintptr_t)a.q | (a.q_stride * 4)) & 15) == 0;
     auto query = [&](int r) {
         const int i = cut.by_group(r);
         return a.q + ((size_t)s.row0 + i) * a.q_stride + (size_t)(head * G + r - i * G) * HD;
     };
     auto rope = [&](int r) { return pl.rope32 ? pl.rope32 + ((size_t)s.row0 + cut.by_group(r)) * pl.half : nullptr; };
-#pragma unroll
-    for (int u = 0; u < R; u++) {
-        const int r = min(row0 + 16 * u + q16, rows - 1);
-        pos[u] = s.past + cut.by_group(r);
-        w0[u] = a.window && a.window <= pos[u] ? pos[u] - a.window + 1 : 0;
-    }
+    const int own = min(row0 + q16, rows - 1);  // the lane's row
+    const int pos = s.past + cut.by_group(own), w0 = a.window && a.window <= pos ? pos - a.window + 1 : 0;
     if constexpr (PAGES) {
         // Once for the workgroup, HD / 16 consecutive dimensions a thread (16 lanes
-        // are a row), handed over in the operand's order.  (Every wavefront for
-        // itself: 64 lanes in as many cache lines for each load, 27.8 us instead of
-        // 32.8 for 48 chats.)
+        // are a row), handed over in the operand's order.  (By every wavefront for
+        // itself a load's 64 lanes are in as many cache lines: 33 us instead of 28
+        // for 48 chats.)
         constexpr int E = HD / 16;
-        static_assert(256 * R <= NW * 64, "a thread has one piece of the rows");
-        if (threadIdx.x < 256 * R) {
-            const int u = threadIdx.x >> 8, e0 = (threadIdx.x & 15) * E, k = (threadIdx.x >> 4) & 15, r = row0 + 16 * u + k;
+        static_assert(NW >= 4, "a thread has one piece of the rows");
+        if (threadIdx.x < 256) {
+            const int e0 = (threadIdx.x & 15) * E, k = threadIdx.x >> 4, r = row0 + k;
             float x[E] = {};
             float amax = 0.0f, c = 0.0f;
             bool ok = true;
@@ -283,63 +293,52 @@ __global__ __launch_bounds__(NW * 64, PAGES ? (HD == 64 ? 3 : 2) : (HD == 64 ? 4
                 for (int e = 0; e < E; e++) amax = fmaxf(amax, fabsf(x[e]));
             }
             const int shift = query_shift(sq_row_max(ok ? amax : INFINITY), scale, c);
-            if ((threadIdx.x & 15) == 0) s_cq[u * 16 + k] = c;
+            if ((threadIdx.x & 15) == 0) s_cq[k] = c;
             // dimension d: chunk d / 64, lane group (d / 16) % 4, half (d / 8) % 2
-            const int at = (((u * C + (e0 >> 6)) * 2 + ((e0 >> 3) & 1)) * 64 + ((e0 >> 4) & 3) * 16 + k) * 8 + (e0 & 7);
+            const int at = (((e0 >> 6) * 2 + ((e0 >> 3) & 1)) * 64 + ((e0 >> 4) & 3) * 16 + k) * 8 + (e0 & 7);
 #pragma unroll
             for (int e = 0; e < E; e++) halves(x[e], shift, s_q[0][at + e], s_q[1][at + e]);
         }
         __syncthreads();
+        cq = s_cq[q16];
 #pragma unroll
-        for (int u = 0; u < R; u++) {
-            cq[u] = s_cq[u * 16 + q16];
+        for (int c = 0; c < C; c++)
 #pragma unroll
-            for (int c = 0; c < C; c++)
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    qh[u][c][h] = *(const v8h*)&s_q[0][(((u * C + c) * 2 + h) * 64 + lane) * 8];
-                    ql[u][c][h] = *(const v8h*)&s_q[1][(((u * C + c) * 2 + h) * 64 + lane) * 8];
-                }
-        }
-    } else {
-#pragma unroll
-        for (int u = 0; u < R; u++) {
-            const int r = min(row0 + 16 * u + q16, rows - 1);
-            float x[C][16];
-            float amax = 0.0f;
-            bool ok = true;
-#pragma unroll
-            for (int c = 0; c < C; c++) {
-                ok = load_query<16>(query(r), vec, rope(r), pl.half, 64 * c + 16 * g, x[c]) && ok;
-#pragma unroll
-                for (int e = 0; e < 16; e++) amax = fmaxf(amax, fabsf(x[c][e]));
+            for (int h = 0; h < 2; h++) {
+                qh[c][h] = *(const v8h*)&s_q[0][((c * 2 + h) * 64 + lane) * 8];
+                ql[c][h] = *(const v8h*)&s_q[1][((c * 2 + h) * 64 + lane) * 8];
             }
-            const int shift = query_shift(groups_max(ok ? amax : INFINITY), scale, cq[u]);
+    } else {
+        float x[C][16];
+        float amax = 0.0f;
+        bool ok = true;
 #pragma unroll
-            for (int c = 0; c < C; c++)
+        for (int c = 0; c < C; c++) {
+            ok = load_query<16>(query(own), vec, rope(own), pl.half, 64 * c + 16 * g, x[c]) && ok;
 #pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    _Float16 h, lo;
-                    halves(x[c][e], shift, h, lo);
-                    qh[u][c][e / 8][e % 8] = h, ql[u][c][e / 8][e % 8] = lo;
-                }
+            for (int e = 0; e < 16; e++) amax = fmaxf(amax, fabsf(x[c][e]));
         }
+        const int shift = query_shift(groups_max(ok ? amax : INFINITY), scale, cq);
+#pragma unroll
+        for (int c = 0; c < C; c++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                _Float16 h, lo;
+                halves(x[c][e], shift, h, lo);
+                qh[c][e / 8][e % 8] = h, ql[c][e / 8][e % 8] = lo;
+            }
     }
 
     // (-1 that the compiler does not know to be: p - h then takes the f16 half as it
     // is, where it would convert it to f32 first)
     float minus = -1.0f;
     asm volatile("" : "+v"(minus));
-    v4f o[R][DT];
-    float m[R], l[R];
+    v4f o[DT];
+    float m = -INFINITY, l = 0.0f;
 #pragma unroll
-    for (int t = 0; t < R; t++) {
-        m[t] = -INFINITY, l[t] = 0.0f;
-#pragma unroll
-        for (int d = 0; d < DT; d++) o[t][d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    }
+    for (int d = 0; d < DT; d++) o[d] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
     // rows between the tile's first and last position see a page whole where both do
-    const int pos_lo = s.past + cut.by_group(row0), pos_hi = s.past + cut.by_group(min(rows, row0 + 16 * R) - 1);
+    const int pos_lo = s.past + cut.by_group(row0), pos_hi = s.past + cut.by_group(min(rows, row0 + 16) - 1);
     const int w0_hi = a.window && a.window <= pos_hi ? pos_hi - a.window + 1 : 0;
 
     int turn = 0;
@@ -369,88 +368,77 @@ __global__ __launch_bounds__(NW * 64, PAGES ? (HD == 64 ? 3 : 2) : (HD == 64 ? 4
                 return s_kv[turn][(e * 2 + h) * 64 + lane];
         };
         // scores [tile of 16 positions][position 4 g + r]
-        v4f x[R][4];
+        v4f x[4];
 #pragma unroll
         for (int t = 0; t < 4; t++) {
-#pragma unroll
-            for (int u = 0; u < R; u++) x[u][t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+            x[t] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int c = 0; c < C; c++) {
                 const v8h k0 = half(t * C + c, 0), k1 = half(t * C + c, 1);
-#pragma unroll
-                for (int u = 0; u < R; u++) {
-                    x[u][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, ql[u][c][0], x[u][t], 0, 0, 0);
-                    x[u][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, ql[u][c][1], x[u][t], 0, 0, 0);
-                    x[u][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qh[u][c][0], x[u][t], 0, 0, 0);
-                    x[u][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, qh[u][c][1], x[u][t], 0, 0, 0);
-                }
+                x[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, ql[c][0], x[t], 0, 0, 0);
+                x[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, ql[c][1], x[t], 0, 0, 0);
+                x[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k0, qh[c][0], x[t], 0, 0, 0);
+                x[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k1, qh[c][1], x[t], 0, 0, 0);
             }
         }
         const bool full = (page + 1) * kPage - 1 <= pos_lo && (page * kPage >= w0_hi || (page + 1) * kPage <= a.sinks);
         const float vs = page_unit(sc.y, unit), lr = __builtin_amdgcn_logf(vs), back = unit / vs;
-        v8h ph[R][2], plo[R][2];
-#pragma unroll
-        for (int u = 0; u < R; u++) {
-            float cs = cq[u] * sc.x;
-            if (!full) {
-#pragma unroll
-                for (int t = 0; t < 4; t++)
-#pragma unroll
-                    for (int r = 0; r < 4; r++) {
-                        const int at = page * kPage + 16 * t + 4 * g + r;
-                        const bool hidden = (at > pos[u]) | ((at < w0[u]) & (at >= a.sinks));
-                        x[u][t][r] = hidden ? -INFINITY : x[u][t][r] * cs;
-                    }
-                cs = 1.0f;
-            }
-            float mx = -INFINITY;
+        float cs = cq * sc.x;
+        if (!full) {
 #pragma unroll
             for (int t = 0; t < 4; t++)
 #pragma unroll
-                for (int r = 0; r < 4; r++) mx = fmaxf(mx, x[u][t][r]);
-            mx = mx * cs + lr;
-            if (__any(mx > m[u] + kHeadroom)) {
-                const float mn = fmaxf(m[u], groups_max(mx));
-                const float alpha = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m[u] - mn);
-                m[u] = mn;
-                l[u] *= alpha;
-#pragma unroll
-                for (int d = 0; d < DT; d++) o[u][d] *= alpha;
-            }
-            const float off = kBase - (m[u] == -INFINITY ? 0.0f : m[u]) + lr;
-            float sum = 0.0f;
-#pragma unroll
-            for (int r = 0; r < 4; r++)
-#pragma unroll
-                for (int t = 0; t < 4; t += 2) {
-                    const v2f p = {__builtin_amdgcn_exp2f(fmaf(x[u][t][r], cs, off)),
-                                   __builtin_amdgcn_exp2f(fmaf(x[u][t + 1][r], cs, off))};
-                    sum += p[0] + p[1];
-                    const v2h h = __builtin_convertvector(p, v2h);
-                    const v2f rest = {fmaf((float)h[0], minus, p[0]), fmaf((float)h[1], minus, p[1])};
-                    const v2h w = __builtin_convertvector(rest, v2h);
-                    const int j = 4 * r + t;
-                    ph[u][j / 8][j % 8] = h[0], ph[u][j / 8][j % 8 + 1] = h[1];
-                    plo[u][j / 8][j % 8] = w[0], plo[u][j / 8][j % 8 + 1] = w[1];
+                for (int r = 0; r < 4; r++) {
+                    const int at = page * kPage + 16 * t + 4 * g + r;
+                    const bool hidden = (at > pos) | ((at < w0) & (at >= a.sinks));
+                    x[t][r] = hidden ? -INFINITY : x[t][r] * cs;
                 }
-            l[u] += sum * back;
+            cs = 1.0f;
         }
+        float mx = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < 4; t++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) mx = fmaxf(mx, x[t][r]);
+        mx = mx * cs + lr;
+        if (__any(mx > m + kHeadroom)) {
+            const float mn = fmaxf(m, groups_max(mx));
+            const float alpha = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= alpha;
+#pragma unroll
+            for (int d = 0; d < DT; d++) o[d] *= alpha;
+        }
+        const float off = kBase - (m == -INFINITY ? 0.0f : m) + lr;
+        float sum = 0.0f;
+        v8h ph[2], plo[2];
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+#pragma unroll
+            for (int t = 0; t < 4; t += 2) {
+                const v2f p = {__builtin_amdgcn_exp2f(fmaf(x[t][r], cs, off)),
+                               __builtin_amdgcn_exp2f(fmaf(x[t + 1][r], cs, off))};
+                sum += p[0] + p[1];
+                const v2h h = __builtin_convertvector(p, v2h);
+                const v2f rest = {fmaf((float)h[0], minus, p[0]), fmaf((float)h[1], minus, p[1])};
+                const v2h w = __builtin_convertvector(rest, v2h);
+                const int j = 4 * r + t;
+                ph[j / 8][j % 8] = h[0], ph[j / 8][j % 8 + 1] = h[1];
+                plo[j / 8][j % 8] = w[0], plo[j / 8][j % 8 + 1] = w[1];
+            }
+        l += sum * back;
         if (PAGES && more) {
             locate(id);
             load(0, 4 * C);
             id = number(i + 2 * step);
         }
-        auto weigh = [&](int u, v8h v0, v8h v1, v4f y) {
-            y = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, plo[u][0], y, 0, 0, 0);
-            y = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, plo[u][1], y, 0, 0, 0);
-            y = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, ph[u][0], y, 0, 0, 0);
-            return __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, ph[u][1], y, 0, 0, 0);
-        };
 #pragma unroll
         for (int d = 0; d < DT; d++) {
             const v8h v0 = half(4 * C + d, 0), v1 = half(4 * C + d, 1);
-#pragma unroll
-            for (int u = 0; u < R; u++) o[u][d] = weigh(u, v0, v1, o[u][d]);
+            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, plo[0], o[d], 0, 0, 0);
+            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, plo[1], o[d], 0, 0, 0);
+            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v0, ph[0], o[d], 0, 0, 0);
+            o[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v1, ph[1], o[d], 0, 0, 0);
         }
         if constexpr (PAGES) {
             if (more) load(4 * C, P);
@@ -465,8 +453,7 @@ __global__ __launch_bounds__(NW * 64, PAGES ? (HD == 64 ? 3 : 2) : (HD == 64 ? 4
             __syncthreads();
         }
     }
-#pragma unroll
-    for (int u = 0; u < R; u++) l[u] = groups_sum(l[u]);
+    l = groups_sum(l);
 
     // where four of row r's sums go: its output, or its part of the workspace
     const bool vec_out = (((uintptr_t)a.out | (a.out_stride * 4)) & 15) == 0;
@@ -490,27 +477,24 @@ __global__ __launch_bounds__(NW * 64, PAGES ? (HD == 64 ? 3 : 2) : (HD == 64 ? 4
     };
     if constexpr (PAGES) {
         // (a wavefront that saw nothing has no weight; NaN scores keep their NaN)
+        if (row0 + q16 < rows) {
+            const int k = wave * 16 + q16;
+            if (g == 0) s_m[k] = m, s_l[k] = l;
 #pragma unroll
-        for (int u = 0; u < R; u++) {
-            const int r = 16 * u + q16, k = wave * 16 * R + r;
-            if (row0 + r < rows) {
-                if (g == 0) s_m[k] = m[u], s_l[k] = l[u];
-#pragma unroll
-                for (int d = 0; d < DT; d++) *(v4f*)&s_o[k * (HD + 4) + 16 * d + 4 * g] = o[u][d];
-            }
+            for (int d = 0; d < DT; d++) *(v4f*)&s_o[k * (HD + 4) + 16 * d + 4 * g] = o[d];
         }
         __syncthreads();
-        for (int e = threadIdx.x; e < 16 * R * (HD / 4); e += NW * 64) {
+        for (int e = threadIdx.x; e < 16 * (HD / 4); e += NW * 64) {
             const int r = e / (HD / 4), d = e % (HD / 4) * 4;
             if (row0 + r >= rows) break;
             float mm = -INFINITY, ll = 0.0f;
             v4f v = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int w = 0; w < NW; w++) mm = fmaxf(mm, s_m[w * 16 * R + r]);
+            for (int w = 0; w < NW; w++) mm = fmaxf(mm, s_m[w * 16 + r]);
             const float base = mm == -INFINITY ? 0.0f : mm;
 #pragma unroll
             for (int w = 0; w < NW; w++) {
-                const int k = w * 16 * R + r;
+                const int k = w * 16 + r;
                 const float m1 = s_m[k], l1 = s_l[k];
                 const float f = __builtin_amdgcn_exp2f((m1 == -INFINITY && l1 != 0.0f ? 0.0f : m1) - base);
                 ll += l1 * f;
@@ -518,24 +502,20 @@ __global__ __launch_bounds__(NW * 64, PAGES ? (HD == 64 ? 3 : 2) : (HD == 64 ? 4
             }
             emit(row0 + r, d, v, mm, ll);
         }
-    } else {
+    } else if (row0 + q16 < rows) {
 #pragma unroll
-        for (int u = 0; u < R; u++) {
-            const int r = row0 + 16 * u + q16;
-            if (r >= rows) continue;
-#pragma unroll
-            for (int d = 0; d < DT; d++) emit(r, 16 * d + 4 * g, o[u][d], m[u], l[u]);
-        }
+        for (int d = 0; d < DT; d++) emit(own, 16 * d + 4 * g, o[d], m, l);
     }
 }
 
 // The parts of the rows whose pages were cut, from (sequence, KV head, row).
 // W wavefronts share a row: all four of a workgroup where rows are few and parts
-// many (131000 positions: 32 rows of 21 parts), one where it is the other way.
+// many (131000 positions: 32 rows of 93 parts, 5 us), one where it is the other way.
 // The lanes find the factors of 64 parts, then a wavefront adds every W-th
 // part, eight in flight at a time.
 template <int HD, int W>
-__global__ __launch_bounds__(256) void sdpa_merge_kernel(KvView kv, KvPlanView pl, PagedArgs a, Cut cut, int tile_rows) {
+__global__ __launch_bounds__(256) void sdpa_merge_kernel(KvView kv, KvPlanView pl, PagedArgs a, Cut cut,
+                                                         int tile_rows) {
     constexpr int C = HD / 64, IN = 8;
     __shared__ float s_o[4][HD];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, mine = wave % W;
@@ -546,7 +526,8 @@ __global__ __launch_bounds__(256) void sdpa_merge_kernel(KvView kv, KvPlanView p
     int parts = 1;
     if (rows >= cut.rows_lo && rows <= cut.rows_hi && r < rows) {
         const int tile = r / tile_rows, row_end = min(rows, (tile + 1) * tile_rows);
-        const Span span = tile_span(s.past + cut.by_group(tile * tile_rows), s.past + cut.by_group(row_end - 1), a.window, a.sinks);
+        const Span span =
+            tile_span(s.past + cut.by_group(tile * tile_rows), s.past + cut.by_group(row_end - 1), a.window, a.sinks);
         parts = cut.parts(span.count);
     }
     if (parts == 1) return;  // (W = 4: the whole workgroup)
@@ -570,7 +551,8 @@ __global__ __launch_bounds__(256) void sdpa_merge_kernel(KvView kv, KvPlanView p
 #pragma unroll
             for (int j = 0; j < IN; j++)
 #pragma unroll
-                for (int c = 0; c < C; c++) v[j][c] = k + W * j < n ? w[(i0 + k + W * j) * stride + 64 * c + lane] : 0.0f;
+                for (int c = 0; c < C; c++)
+                    v[j][c] = k + W * j < n ? w[(i0 + k + W * j) * stride + 64 * c + lane] : 0.0f;
 #pragma unroll
             for (int j = 0; j < IN; j++) {
                 const float fj = __builtin_bit_cast(
@@ -637,7 +619,8 @@ Launch plan_launch(const std::vector<KvSeq>& seqs, const KvView& kv, const Paged
         r.cut.tiles = std::max(r.cut.tiles, tiles);
         groups += tiles;
         for (int t = 0; t < tiles; t++) {
-            const Span sp = tile_span(s.past + t * tile / G, s.past + (std::min(rows, (t + 1) * tile) - 1) / G, a.window, a.sinks);
+            const Span sp = tile_span(s.past + t * tile / G, s.past + (std::min(rows, (t + 1) * tile) - 1) / G,
+                                      a.window, a.sinks);
             work += sp.count;
             longest = std::max(longest, sp.count);
         }
@@ -660,7 +643,7 @@ Launch plan_launch(const std::vector<KvSeq>& seqs, const KvView& kv, const Paged
     return r;
 }
 
-template <int HD, int R, int NW, bool PAGES>
+template <int HD, int NW, bool PAGES>
 int launch_one(const Launch& l, const KvView& kv, const KvPlanView& p, const PagedArgs& a) {
     const float scale = 1.4426950408889634f / sqrtf((float)HD);  // scores in units of log 2
     const size_t grid = (size_t)l.cut.tiles * kv.kv_heads;
@@ -668,11 +651,11 @@ int launch_one(const Launch& l, const KvView& kv, const KvPlanView& p, const Pag
     const size_t merge = (size_t)(l.cut.rows_hi * W + 3) / 4 * kv.kv_heads;
     if (!grid_fits(grid, NW * 64) || !grid_fits(merge, 256))
         return set_error(SQ_ERR_SHAPE, "sdpa_paged: ShapeMismatch (too many rows)");
-    hipLaunchKernelGGL((sdpa_paged_kernel<HD, R, NW, PAGES>), dim3((unsigned)grid, l.cut.splits, p.n_seqs),
+    hipLaunchKernelGGL((sdpa_paged_kernel<HD, NW, PAGES>), dim3((unsigned)grid, l.cut.splits, p.n_seqs),
                        dim3(NW * 64), 0, nullptr, kv, p, a, l.cut, scale);
     if (l.cut.splits > 1)
-        hipLaunchKernelGGL((sdpa_merge_kernel<HD, W>), dim3((unsigned)merge, p.n_seqs), dim3(256), 0, nullptr, kv, p, a, l.cut,
-                           PAGES ? 16 * R : NW * 16 * R);
+        hipLaunchKernelGGL((sdpa_merge_kernel<HD, W>), dim3((unsigned)merge, p.n_seqs), dim3(256), 0, nullptr, kv, p, a,
+                           l.cut, PAGES ? 16 : NW * 16);
     return check_launch("sdpa_paged");
 }
 
@@ -688,9 +671,9 @@ int launch_sdpa_paged(const std::vector<KvSeq>& seqs, const KvView& kv, const Kv
         if (!l[many].any) continue;
         l[many].cut.ws = (float*)ws.p;
         if (kv.head_dim == 64)
-            st = many ? launch_one<64, 1, 4, false>(l[1], kv, p, a) : launch_one<64, 1, kFewWaves, true>(l[0], kv, p, a);
+            st = many ? launch_one<64, 4, false>(l[1], kv, p, a) : launch_one<64, kFewWaves, true>(l[0], kv, p, a);
         else
-            st = many ? launch_one<128, 1, 4, false>(l[1], kv, p, a) : launch_one<128, 1, kFewWaves, true>(l[0], kv, p, a);
+            st = many ? launch_one<128, 4, false>(l[1], kv, p, a) : launch_one<128, kFewWaves, true>(l[0], kv, p, a);
     }
     return st;
 }

