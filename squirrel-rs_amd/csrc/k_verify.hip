@@ -244,7 +244,7 @@ __device__ __forceinline__ Choice choose(const VerifyBatch& b, const VerifyArgs&
         if (i <= n) c = examine(a, target_rows, chunks, parts, t0 + i, d0 + min(i, n - 1), i == n, i, stop);
         if ((threadIdx.x & 63) == 0) s_c[wave] = c, s_stop[wave] = stop;
         __syncthreads();
-        // (i <= n = the last one's own stop: some round has one)
+        // (the row behind the last draft always stops)
         for (int w = 0; w < kWaves; w++)
             if (s_stop[w]) return s_c[w];
         __syncthreads();
