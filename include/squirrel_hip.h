@@ -296,9 +296,10 @@ int sq_kv_plan_new(const sq_kv_pool* pool, sq_kv_plan** out);
  * at least the pages of past[i] + n_new[i] positions.  The batch's rows are
  * sequence 0's, then sequence 1's, and so on.  A page past the pool, or one
  * that the step writes and that stands in the tables a second time, is
- * SQ_ERR_ARG (pages that are only read may be shared).  past[i] may be less
- * than an earlier step left: drafts that were rejected are overwritten.  A
- * refused call leaves the plan's former step in place. */
+ * SQ_ERR_ARG (pages that are only read may be shared; one that is written changes
+ * for whoever else holds it).  At most 65535 sequences and 524287 rows.  past[i]
+ * may be less than an earlier step left: drafts that were rejected are
+ * overwritten.  A refused call leaves the plan's former step in place. */
 int sq_kv_plan_set(sq_kv_plan* plan, size_t n_seqs, const uint32_t* past, const uint32_t* n_new,
                    const uint32_t* tables, size_t table_stride);
 void sq_kv_plan_free(sq_kv_plan* plan);

@@ -189,7 +189,7 @@ __device__ __forceinline__ void halves(float x, int shift, _Float16& h, _Float16
 // 8192 rows of 32 heads of 64 (two f16 products for one of f32: 577 at the rate
 // of a large f16 product), and about 12 us of start and end: 50 us for 1531
 // rows behind 517.
-constexpr int kStat = 4;  // floats behind a part's sums: the maximum, the sum of weights, two unused
+constexpr int kStat = 4;  // floats behind a part's sums: the maximum, the sum of weights, the unit, none
 constexpr float kBase = 8.0f, kHeadroom = 6.0f;
 template <int HD, int NW, bool PAGES>
 __global__ __launch_bounds__(NW * 64, HD != 64 ? 2 : PAGES ? 3 : 4) void sdpa_paged_kernel(KvView kv, KvPlanView pl,
@@ -472,7 +472,7 @@ __global__ __launch_bounds__(NW * 64, HD != 64 ? 2 : PAGES ? 3 : 4) void sdpa_pa
             const size_t at = (cut.slot(s, seq, part) * kv.kv_heads + head) * cut.rows_hi + r;
             float* w = cut.ws + at * (HD + kStat);
             *(v4f*)(w + d) = v;
-            if (d == 0) *(v2f*)(w + HD) = v2f{mm, ll};
+            if (d == 0) *(v4f*)(w + HD) = v4f{mm, ll, unit, 0.0f};
         }
     };
     if constexpr (PAGES) {
@@ -531,28 +531,37 @@ __global__ __launch_bounds__(256) void sdpa_merge_kernel(KvView kv, KvPlanView p
         parts = cut.parts(span.count);
     }
     if (parts == 1) return;  // (W = 4: the whole workgroup)
-    const float unit = first_unit(kv.scales[(size_t)pl.pages[s.table0] * kv.kv_heads + head].y);
     const size_t stride = (size_t)kv.kv_heads * cut.rows_hi * (HD + kStat);
     const float* w = cut.ws + ((cut.slot(s, seq, 0) * kv.kv_heads + head) * cut.rows_hi + r) * (HD + kStat);
-    float mm = -INFINITY, ll = 0.0f, o[C] = {};
-    for (int i = lane; i < parts; i += 64) mm = fmaxf(mm, w[i * stride + HD]);
+    // part i's maximum, sum of weights and unit; its sums and those of the next IN - 1
+    // that are this wavefront's
+    auto stat = [&](int i) {
+        return i < parts ? *(const v4f*)(w + i * stride + HD) : v4f{-INFINITY, 0.0f, 0.0f, 0.0f};
+    };
+    float v[IN][C];
+    auto sums = [&](int i, int end) {
+#pragma unroll
+        for (int j = 0; j < IN; j++)
+#pragma unroll
+            for (int c = 0; c < C; c++)
+                v[j][c] = i + W * j < end ? w[(i + W * j) * stride + 64 * c + lane] : 0.0f;
+    };
+    v4f st = stat(lane);
+    const float mine_unit = st[2];  // (a bit cast of a vector's element would take its first)
+    const float unit = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, mine_unit), 0));
+    sums(mine, min(parts, 64));  // (in flight while the factors form)
+    float mm = st[0], ll = 0.0f, o[C] = {};
+    for (int i = lane + 64; i < parts; i += 64) mm = fmaxf(mm, stat(i)[0]);
     mm = sq_wave_max(mm);
     for (int i0 = 0; i0 < parts; i0 += 64) {
-        float f = 0.0f;
-        if (i0 + lane < parts) {
-            const float m1 = w[(i0 + lane) * stride + HD], l1 = w[(i0 + lane) * stride + HD + 1];
-            // (a part that saw nothing adds nothing; NaN scores keep their NaN)
-            f = __builtin_amdgcn_exp2f((m1 == -INFINITY && l1 != 0.0f ? 0.0f : m1) - (mm == -INFINITY ? 0.0f : mm));
-            ll += l1 * f;
-        }
+        if (i0) st = stat(i0 + lane);
+        // (a part that saw nothing adds nothing; NaN scores keep their NaN)
+        const float f = __builtin_amdgcn_exp2f((st[0] == -INFINITY && st[1] != 0.0f ? 0.0f : st[0]) -
+                                               (mm == -INFINITY ? 0.0f : mm));
+        ll += st[1] * f;
         const int n = min(parts - i0, 64);
         for (int k = mine; k < n; k += W * IN) {
-            float v[IN][C];
-#pragma unroll
-            for (int j = 0; j < IN; j++)
-#pragma unroll
-                for (int c = 0; c < C; c++)
-                    v[j][c] = k + W * j < n ? w[(i0 + k + W * j) * stride + 64 * c + lane] : 0.0f;
+            if (i0 + k != mine) sums(i0 + k, i0 + n);
 #pragma unroll
             for (int j = 0; j < IN; j++) {
                 const float fj = __builtin_bit_cast(

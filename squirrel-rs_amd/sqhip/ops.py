@@ -5,6 +5,7 @@ reference's op does and raises KernelError with the same kind on failure.
 """
 from __future__ import annotations
 
+import bisect
 import ctypes as C
 
 import numpy as np
@@ -238,7 +239,8 @@ class KvPlan:
     before it, rows of it, and the page table of each."""
 
     def __init__(self, pool: KvPool, past=None, new=None, tables=None):
-        self.pool, self.rows, self.lengths, self.h = pool, 0, np.zeros(0, np.int64), None
+        self.pool, self.rows, self.h = pool, 0, None
+        self._lengths, self._sums = [], [0]
         h = C.c_void_p()
         check(lib().sq_kv_plan_new(pool.h, C.byref(h)))
         self.h = h.value
@@ -254,7 +256,14 @@ class KvPlan:
                 _shape_error()
         p, n, t = (np.ascontiguousarray(a, dtype=np.uint32) for a in (past, new, tables))
         check(lib().sq_kv_plan_set(self.h, len(p), p.ctypes.data, n.ctypes.data, t.ctypes.data, t.shape[1]))
-        self.rows, self.lengths = int(n.astype(np.int64).sum()), p.astype(np.int64) + n
+        self.rows = int(n.astype(np.int64).sum())
+        lengths = np.sort(p.astype(np.int64) + n)
+        self._lengths, self._sums = lengths.tolist(), [0, *np.cumsum(lengths).tolist()]
+
+    def cached_rows(self, last: int) -> int:
+        """Rows that kv_read gives: the last `last` positions of every sequence."""
+        short = bisect.bisect_left(self._lengths, last)
+        return self._sums[short] + last * (len(self._lengths) - short)
 
     def __del__(self):
         try:
@@ -285,7 +294,9 @@ def kv_append(plan: KvPlan, layer: int, k: DeviceArray, v: DeviceArray, rotated:
 
 def kv_read(plan: KvPlan, layer: int, last: int, k: DeviceArray, v: DeviceArray) -> None:
     """The cached values of each sequence's last `last` positions (sq_kv_read)."""
-    n = int(np.minimum(plan.lengths, last).sum()) * plan.pool.n_kv_heads * plan.pool.head_dim
+    if last < 0:
+        _shape_error()
+    n = plan.cached_rows(last) * plan.pool.n_kv_heads * plan.pool.head_dim
     if k.size != n or v.size != n:
         _shape_error()
     check(lib().sq_kv_read(plan.h, layer, last, k.ptr, v.ptr))

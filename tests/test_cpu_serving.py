@@ -17,7 +17,7 @@ def emulated():
     return build_emu_lib.build()
 
 
-@pytest.mark.parametrize("tests", ["refusals or nothing", "append or growing or partial or far or zero_and or apart",
+@pytest.mark.parametrize("tests", ["refusals or nothing or read_sizes", "append or growing or partial or far or zero_and or apart",
                                    "layers or finite or flat or rotated or bad_queries or batch or very_different",
                                    "test_sdpa_paged",
                                    "verify or rejection", "serving_steps"])

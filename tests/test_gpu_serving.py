@@ -493,6 +493,20 @@ def test_refusals_small():
     t.check_cache(plan, [0, 0], [70, 70])
 
 
+def test_read_sizes_small():
+    """What kv_read gives for any `last`, and its refusals."""
+    past, new = [3, 0, 100], [1, 0, 30]
+    t = Step([4, 1, 130], 1, 64, seed=22)
+    t.append([0, 0, 0], past)
+    plan = t.append(past, new)
+    for last in (0, 1, 4, 5, 129, 130, 1 << 40):
+        assert plan.cached_rows(last) == sum(min(a + b, last) for a, b in zip(past, new))
+        t.check_cache(plan, past, new, last=last)
+    for last in (-1, 3):
+        with pytest.raises(KernelError):
+            ops.kv_read(plan, 0, last, DeviceArray((5, 64)), DeviceArray((5, 64)))
+
+
 def test_steps_with_nothing_to_do_small():
     """No sequences, no rows, an unset plan: nothing runs, nothing is refused."""
     t = Step([10], 1, 64, seed=21)
